@@ -56,6 +56,14 @@ SIGNATURES = {
     "cula_kda_short_conv_bwd": (_i, [_vp, _fp, _fp, _fp, _vp, _vp, _fp, _fp, _ip, _ip, _i, _i, _i, _i, _i, _vp]),
     "cula_kda_rms_norm_gated_fwd": (_i, [_vp, _vp, _fp, _vp, _fp, ctypes.c_longlong, _i, _i, _f, _vp]),
     "cula_kda_rms_norm_gated_bwd": (_i, [_vp, _vp, _fp, _fp, _vp, _vp, _vp, _fp, ctypes.c_longlong, _i, _i, _vp]),
+    "cula_kda_selective_scan_fwd": (_i, [_vp, _vp]),
+    "cula_kda_selective_scan_bwd": (_i, [_vp, _vp]),
+    "cula_kda_selective_scan_tiles": (_i, [_i, _i, _i]),
+    "cula_kda_selective_step": (_i, [_vp, _vp]),
+    "cula_kda_conv_step": (_i, [_vp, _vp]),
+    "cula_kda_add_rms_norm_fwd": (_i, [_vp, _vp]),
+    "cula_kda_add_rms_norm_bwd": (_i, [_vp, _vp]),
+    "cula_kda_add_rms_norm_shares": (_i, [_i, ctypes.c_longlong]),
     "cula_kda_selftest_bounded_wait": (_i, [_ip, _i, _vp]),
     "cula_kda_strerror": (ctypes.c_char_p, [_i]),
 }

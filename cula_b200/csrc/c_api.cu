@@ -476,6 +476,103 @@ extern "C" int cula_kda_rms_norm_gated_bwd(const void* d_x, const void* d_g, con
     return rc == -1 ? CULA_KDA_EINVAL : rc;
 }
 
+extern "C" int kda_launch_selective_scan_fwd(const kda::SelScanArgs* a, int state_lanes, cudaStream_t stream);
+extern "C" int kda_launch_selective_scan_bwd(const kda::SelScanArgs* a, int state_lanes, cudaStream_t stream);
+extern "C" int kda_selective_scan_tiles(int D, int groups, int state_lanes);
+extern "C" int kda_launch_selective_step(const kda::SelStepArgs* a, cudaStream_t stream);
+extern "C" int kda_launch_conv_step(const kda::ConvStepArgs* a, cudaStream_t stream);
+extern "C" int kda_launch_add_rms_norm(const kda::AddNormArgs* a, int backward, cudaStream_t stream);
+extern "C" int kda_add_rms_norm_shares(int D, long long R);
+
+namespace {
+inline int state_lanes(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
+inline int checked(int rc) { return rc == -1 ? CULA_KDA_EINVAL : rc; }
+int scan_args_error(const kda::SelScanArgs* a) {
+    if (!a || !a->x || !a->dt || !a->Bm || !a->Cm || !a->A || a->D <= 0 || a->G <= 0 || a->S <= 0 || a->S > 64) return CULA_KDA_EINVAL;
+    if (a->D % a->G || a->D / a->G % 8 || a->rows < 0 || a->n_seqs < 0 || a->num_chunks < 0 || a->seg_chunks < 0) return CULA_KDA_EINVAL;
+    const bool packed = a->cu_seqlens != nullptr;
+    if (packed != (a->chunk_indices != nullptr) || packed != (a->chunk_offsets != nullptr) || packed != (a->seq_order != nullptr)) return CULA_KDA_EINVAL;
+    if (packed && (a->total_tokens < 0 || a->total_tokens > a->rows)) return CULA_KDA_EINVAL;
+    if (!packed && a->T < 0) return CULA_KDA_EINVAL;
+    if (a->seg_chunks && (!a->seg_state || !a->seg_dt)) return CULA_KDA_EINVAL;
+    const int per = a->fp32 ? 4 : 8;
+    if (misaligned(a->x) || misaligned(a->dt) || misaligned(a->z) || a->x_row % per || a->dt_row % per || a->x_seq % per || a->dt_seq % per ||
+        (a->z && (a->z_row % per || a->z_seq % per)) || misaligned(a->states) || misaligned(a->seg_state) || misaligned(a->seg_dt) || misaligned(a->y_pre))
+        return CULA_KDA_EALIGN;
+    return 0;
+}
+}
+
+extern "C" int cula_kda_selective_scan_tiles(int D, int G, int S) {
+    return D <= 0 || G <= 0 || S <= 0 || S > 64 ? CULA_KDA_EINVAL : kda_selective_scan_tiles(D, G, state_lanes(S));
+}
+
+extern "C" int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* a, void* stream) {
+    if (const int e = scan_args_error(a)) return e;
+    if (a->n_seqs == 0) return 0;
+    if (!a->y && a->rows) return CULA_KDA_EINVAL;
+    if (a->z && a->states && !a->y_pre && a->rows) return CULA_KDA_EINVAL;
+    if (misaligned(a->y)) return CULA_KDA_EALIGN;
+    return checked(kda_launch_selective_scan_fwd(a, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int cula_kda_selective_scan_bwd(const cula_kda_selective_scan_args* a, void* stream) {
+    if (const int e = scan_args_error(a)) return e;
+    if (a->rows == 0 || a->n_seqs == 0 || a->cta_rows <= 0 || !a->dy || !a->dx || !a->ddt || !a->dBm || !a->dCm || !a->dA || !a->part_bc || !a->part_A ||
+        !a->states || (a->z && (!a->dz || !a->y_pre)) || (a->dskip && !a->part_skip) || (a->dbias && !a->part_bias))
+        return CULA_KDA_EINVAL;
+    if (misaligned(a->dy) || misaligned(a->dx) || misaligned(a->ddt) || misaligned(a->dz) || misaligned(a->part_bc) || misaligned(a->part_A) ||
+        misaligned(a->part_skip) || misaligned(a->part_bias) || misaligned(a->skip) || misaligned(a->dt_bias))
+        return CULA_KDA_EALIGN;
+    return checked(kda_launch_selective_scan_bwd(a, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int cula_kda_selective_step(const cula_kda_selective_step_args* a, void* stream) {
+    if (!a || a->rows < 0) return CULA_KDA_EINVAL;
+    if (a->rows == 0) return 0;
+    if (!a->x || !a->dt || !a->Bm || !a->Cm || !a->A || !a->state || !a->y || !a->status || a->D <= 0 || a->G <= 0 || a->D % a->G || a->S <= 0 || a->S > 64)
+        return CULA_KDA_EINVAL;
+    if (!a->indices && a->pool < a->rows) return CULA_KDA_EINVAL;
+    if (a->vec && (a->S % 4 || misaligned(a->state) || misaligned(a->A))) return CULA_KDA_EALIGN;
+    return checked(kda_launch_selective_step(a, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int cula_kda_conv_step(const cula_kda_conv_step_args* a, void* stream) {
+    if (!a || a->rows < 0) return CULA_KDA_EINVAL;
+    if (a->rows == 0) return 0;
+    if (!a->x || !a->w || !a->cache || !a->y || !a->status || a->D <= 0 || a->D % 8 || a->W < 1 || a->W > 4) return CULA_KDA_EINVAL;
+    if (!a->indices && a->pool < a->rows) return CULA_KDA_EINVAL;
+    if (misaligned(a->w) || misaligned(a->cache) || misaligned(a->y) || (reinterpret_cast<uintptr_t>(a->x) & 3) || a->x_row % 2) return CULA_KDA_EALIGN;
+    return checked(kda_launch_conv_step(a, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int cula_kda_add_rms_norm_shares(int D, long long R) { return D <= 0 || R <= 0 ? 0 : kda_add_rms_norm_shares(D, R); }
+
+static int norm_args_error(const kda::AddNormArgs* a) {
+    if (!a || a->R < 0 || a->D <= 0 || a->D % 8 || a->D > 16384 || a->res < 0 || a->res > 2 || (a->fp32 && a->res == 1)) return CULA_KDA_EINVAL;
+    return 0;
+}
+
+extern "C" int cula_kda_add_rms_norm_fwd(const cula_kda_add_rms_norm_args* a, void* stream) {
+    if (const int e = norm_args_error(a)) return e;
+    if (a->R == 0) return 0;
+    if (!a->x || !a->w || !a->y || (a->res && (!a->r || !a->r_out)) || (a->fp8 && !a->scale)) return CULA_KDA_EINVAL;
+    if (a->fp8 && a->group && ((a->group != 32 && a->group != 64 && a->group != 128 && a->group != 256) || a->D % a->group)) return CULA_KDA_EINVAL;
+    if (misaligned(a->x) || misaligned(a->r) || misaligned(a->w) || misaligned(a->y) || misaligned(a->r_out) || a->x_row % (a->fp32 ? 4 : 8) ||
+        (a->res && a->r_row % (a->res == 2 ? 4 : 8)))
+        return CULA_KDA_EALIGN;
+    return checked(kda_launch_add_rms_norm(a, 0, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int cula_kda_add_rms_norm_bwd(const cula_kda_add_rms_norm_args* a, void* stream) {
+    if (const int e = norm_args_error(a)) return e;
+    if (a->R == 0 || !a->v || !a->w || !a->rstd || !a->dy || !a->dx || !a->part_w || !a->dw) return CULA_KDA_EINVAL;
+    if (misaligned(a->v) || misaligned(a->w) || misaligned(a->dy) || misaligned(a->dr_out) || misaligned(a->dx) || misaligned(a->dr) || misaligned(a->part_w) ||
+        (!a->res && a->x_row % (a->fp32 ? 4 : 8)))
+        return CULA_KDA_EALIGN;
+    return checked(kda_launch_add_rms_norm(a, 1, static_cast<cudaStream_t>(stream)));
+}
+
 extern "C" int kda_launch_selftest_wait(int* status, int limit, cudaStream_t stream);
 
 extern "C" int cula_kda_selftest_bounded_wait(int* d_status, int max_polls, void* stream) {

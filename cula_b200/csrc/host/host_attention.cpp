@@ -539,9 +539,9 @@ void register_node_type() {
 void bind_attention(pybind11::module_& m) {
     namespace py = pybind11;
     py::class_<Tables>(m, "Tables")
-        .def(py::init([](Tensor cu, Tensor ci, Tensor co, Tensor so, int64_t n_seqs, int64_t num_chunks, int64_t total) {
-            return Tables{cu, ci, co, so, n_seqs, num_chunks, total};
-        }));
+        .def(py::init([](Tensor cu, Tensor ci, Tensor co, Tensor so, int64_t n_seqs, int64_t num_chunks, int64_t total, int64_t longest) {
+            return Tables{cu, ci, co, so, n_seqs, num_chunks, total, longest};
+        }), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg("longest") = 0);
     py::class_<Segments>(m, "Segments").def(py::init([](int64_t count, const Tables& t) { return Segments{count, t}; }));
     register_node_type();
     m.def("attend", &attend);

@@ -29,7 +29,9 @@ enum { GATE_NONE = 0, GATE_SOFTPLUS = 1, GATE_LOWER_BOUND = 2 };
     X(cula_kda_decode) X(cula_kda_bwd_scratch_floats) X(cula_kda_bwd_grad_scale) X(cula_kda_bwd_scale_and_intra) X(cula_kda_bwd_scan) X(cula_kda_bwd_both_scans) \
     X(cula_kda_bwd_dense) X(cula_kda_bwd_gated_checked) X(cula_kda_clear) X(cula_kda_gate_fwd) X(cula_kda_gate_bwd)                              \
     X(cula_kda_beta_sigmoid_fwd) X(cula_kda_beta_sigmoid_bwd) X(cula_kda_short_conv_fwd) X(cula_kda_short_conv_bwd)    \
-    X(cula_kda_rms_norm_gated_fwd) X(cula_kda_rms_norm_gated_bwd) X(cula_kda_strerror)
+    X(cula_kda_rms_norm_gated_fwd) X(cula_kda_rms_norm_gated_bwd) X(cula_kda_strerror)                         \
+    X(cula_kda_selective_scan_fwd) X(cula_kda_selective_scan_bwd) X(cula_kda_selective_scan_tiles) X(cula_kda_selective_step)            \
+    X(cula_kda_conv_step) X(cula_kda_add_rms_norm_fwd) X(cula_kda_add_rms_norm_bwd) X(cula_kda_add_rms_norm_shares)
 struct Lib {
 #define CULA_KDA_MEMBER(name) decltype(&::name) name = nullptr;
     CULA_KDA_ENTRIES(CULA_KDA_MEMBER)
@@ -93,10 +95,11 @@ void poll_status(int device_index);
 // the index tables of a packed batch (utils.VarlenTables)
 struct Tables {
     Tensor cu_seqlens, chunk_indices, chunk_offsets, seq_order;
-    int64_t n_seqs = 0, num_chunks = 0, total_tokens = 0;
+    int64_t n_seqs = 0, num_chunks = 0, total_tokens = 0, longest = 0;        // longest: chunks of the longest sequence
 };
 
 void bind_attention(pybind11::module_& m);
 void bind_layer_ops(pybind11::module_& m);
+void bind_ssm(pybind11::module_& m);
 
 }  // namespace cula_host

@@ -78,4 +78,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("status_ptr", [](int dev) { return (int64_t)(intptr_t)cula_host::status_word(dev); });
     cula_host::bind_attention(m);
     cula_host::bind_layer_ops(m);
+    cula_host::bind_ssm(m);
 }

@@ -1,0 +1,353 @@
+// RMS norm with the addition to the residual stream before it, forward and backward, and with an 8-bit output:
+//     v = x + r, rounded to the stream's type (what the next block adds to, and what is normalised);  n = v rsqrt(mean(v^2) + eps);  y = n w
+//     8 bits: per row or per group of columns, scale = max(amax|y| / 448, 2^-126), q = e4m3(y / scale)
+//     dv = rstd (dn - n mean(dn n)) + dr_out with dn = dy w;  dx, dr = dv;  dw = sum over rows of dy n
+// Everything is read and written once: TPR threads hold a row in registers, VPT pieces of 8 columns each.
+#include <cuda_fp8.h>
+
+#include "kda_common.cuh"
+#include "kda_params.h"
+
+namespace kda {
+
+enum { RES_NONE = 0, RES_BF16 = 1, RES_FP32 = 2 };
+constexpr float E4M3_MAX = 448.f, SCALE_MIN = 1.17549435e-38f;
+
+template <typename T> struct Oct;                                   // 8 columns
+template <> struct Oct<__nv_bfloat16> {
+    uint4 r;
+    __device__ void load(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint4*>(p); }
+    __device__ void get(float2 (&v)[4]) const { v[0] = unpack_bf16(r.x); v[1] = unpack_bf16(r.y); v[2] = unpack_bf16(r.z); v[3] = unpack_bf16(r.w); }
+    __device__ void set(const float2 (&v)[4]) {
+        r = make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y), pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
+    }
+    __device__ void store(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = r; }
+};
+template <> struct Oct<float> {
+    float4 a, b;
+    __device__ void load(const float* p) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+    __device__ void get(float2 (&v)[4]) const {
+        v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w); v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
+    }
+    __device__ void set(const float2 (&v)[4]) { a = make_float4(v[0].x, v[0].y, v[1].x, v[1].y); b = make_float4(v[2].x, v[2].y, v[3].x, v[3].y); }
+    __device__ void store(float* p) const { reinterpret_cast<float4*>(p)[0] = a; reinterpret_cast<float4*>(p)[1] = b; }
+};
+template <int RES, typename T> struct StreamOf { using type = T; };
+template <typename T> struct StreamOf<RES_BF16, T> { using type = __nv_bfloat16; };
+template <typename T> struct StreamOf<RES_FP32, T> { using type = float; };
+
+constexpr int norm_threads(int TPR) { return TPR < 128 ? 128 : TPR; }
+
+// the sum (or the maximum of bit patterns) over the TPR threads of a row; `slot` is theirs for this call and not written again before
+// another barrier has passed
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* slot) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TPR > 32) {
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) slot[warp] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) v += slot[w];
+    }
+    return v;
+}
+template <int TPR>
+__device__ __forceinline__ int row_max(int v, int* slot) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if constexpr (TPR > 32) {
+        const int warp = threadIdx.x >> 5;
+        if ((threadIdx.x & 31) == 0) slot[warp] = v;
+        __syncthreads();
+        v = slot[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 32; ++w) v = max(v, slot[w]);
+    }
+    return v;
+}
+
+template <typename T, int RES, bool FP8, int TPR, int VPT>
+__global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_kernel(const AddNormArgs a) {
+    using R = typename StreamOf<RES, T>::type;
+    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR < 32 ? 1 : TPR / 32;
+    __shared__ float s_sum[2][WARPS];
+    __shared__ int s_max[2][WARPS];
+    const int lane = threadIdx.x % TPR, nv = a.D / 8;
+    pdl_launch_dependents();
+    pdl_wait();
+    Oct<float> w[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+        if (const int c = lane + v * TPR; c < nv) w[v].load(a.w + 8 * c);
+    int parity = 0;
+    for (long long row = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR; row - threadIdx.x / TPR < a.R; row += (long long)gridDim.x * GROUPS, parity ^= 1) {
+        const bool live = row < a.R;
+        Oct<T> rx[VPT];
+        Oct<R> rr[VPT];
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                rx[v].load(static_cast<const T*>(a.x) + row * a.x_row + 8 * c);
+                if (RES != RES_NONE) rr[v].load(static_cast<const R*>(a.r) + row * a.r_row + 8 * c);
+            }
+        }
+        float2 val[VPT][4], ss = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                rx[v].get(val[v]);
+                if constexpr (RES != RES_NONE) {
+                    float2 r[4];
+                    rr[v].get(r);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) val[v][e] = add2(val[v][e], r[e]);
+                    rr[v].set(val[v]);                               // the one rounding of the stream: what is kept is what is normalised
+                    rr[v].store(static_cast<R*>(a.r_out) + (size_t)row * a.D + 8 * c);
+                    rr[v].get(val[v]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ss = fma2(val[v][e], val[v][e], ss);
+            }
+        }
+        const float rstd = rsqrtf(row_sum<TPR>(ss.x + ss.y, s_sum[parity]) * (1.f / a.D) + a.eps);
+        if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
+        int top = 0;                                                 // bits of the largest |y|: a NaN is larger than anything
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                float2 wv[4];
+                if constexpr (TPR * VPT > 1024) w[v].load(a.w + 8 * c);          // too many to be held
+                w[v].get(wv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) val[v][e] = mul2(mul2(val[v][e], splat2(rstd)), wv[e]);
+                if constexpr (!FP8) {
+                    Oct<T> o;
+                    o.set(val[v]);
+                    o.store(static_cast<T*>(a.y) + (size_t)row * a.D + 8 * c);
+                }
+            }
+        }
+        if constexpr (FP8) {
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = lane + v * TPR;
+                int m = 0;
+                if (live && c < nv) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = max(m, max(__float_as_int(fabsf(val[v][e].x)), __float_as_int(fabsf(val[v][e].y))));
+                }
+                if (a.group) {                                       // the threads of a group are neighbours in one warp
+                    for (int o = a.group / 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    if (live && c < nv) {
+                        const float amax = __int_as_float(m) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax, inv = 1.f / scale;
+                        if (8 * c % a.group == 0) a.scale[row * (a.D / a.group) + 8 * c / a.group] = scale;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) val[v][e] = mul2(val[v][e], splat2(inv));
+                    }
+                } else top = max(top, m);
+            }
+            if (!a.group) {
+                const float amax = __int_as_float(row_max<TPR>(top, s_max[parity])) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax, inv = 1.f / scale;
+                if (live && lane == 0) a.scale[row] = scale;
+#pragma unroll
+                for (int v = 0; v < VPT; ++v)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) val[v][e] = mul2(val[v][e], splat2(inv));
+            }
+#pragma unroll
+            for (int v = 0; v < VPT; ++v) {
+                const int c = lane + v * TPR;
+                if (live && c < nv) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[e] = __nv_cvt_float2_to_fp8x2(val[v][e], __NV_SATFINITE, __NV_E4M3);
+                    *reinterpret_cast<uint2*>(static_cast<unsigned char*>(a.y) + (size_t)row * a.D + 8 * c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int RES, int TPR, int VPT>
+__global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_bwd_kernel(const AddNormArgs a) {
+    using R = typename StreamOf<RES, T>::type;
+    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR < 32 ? 1 : TPR / 32;
+    __shared__ float s_sum[2][WARPS];
+    const int lane = threadIdx.x % TPR, nv = a.D / 8;
+    const long long group = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR;
+    pdl_launch_dependents();
+    pdl_wait();
+    float2 dw[VPT][4];
+    Oct<float> w[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int c = lane + v * TPR;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dw[v][e] = make_float2(0.f, 0.f);
+        if (c < nv) w[v].load(a.w + 8 * c);
+    }
+    int parity = 0;
+    for (long long row = group; row - threadIdx.x / TPR < a.R; row += (long long)gridDim.x * GROUPS, parity ^= 1) {
+        const bool live = row < a.R;
+        Oct<R> rv[VPT], rd[VPT];
+        Oct<T> ry[VPT];
+        const float rstd = live ? a.rstd[row] : 0.f;
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                const size_t at = (size_t)row * a.D + 8 * c;
+                rv[v].load(static_cast<const R*>(a.v) + (RES == RES_NONE ? row * a.x_row + 8 * c : at));
+                ry[v].load(static_cast<const T*>(a.dy) + at);
+                if (RES != RES_NONE && a.dr_out) rd[v].load(static_cast<const R*>(a.dr_out) + at);
+            }
+        }
+        float2 n[VPT][4], dn[VPT][4], dot = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                float2 dy[4], wv[4];
+                if constexpr (TPR * VPT > 1024) w[v].load(a.w + 8 * c);          // too many to be held
+                w[v].get(wv);
+                rv[v].get(n[v]);
+                ry[v].get(dy);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    n[v][e] = mul2(n[v][e], splat2(rstd));
+                    dw[v][e] = fma2(dy[e], n[v][e], dw[v][e]);
+                    dn[v][e] = mul2(dy[e], wv[e]);
+                    dot = fma2(dn[v][e], n[v][e], dot);
+                }
+            }
+        }
+        const float m = -row_sum<TPR>(dot.x + dot.y, s_sum[parity]) * (1.f / a.D);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) {
+            const int c = lane + v * TPR;
+            if (live && c < nv) {
+                const size_t at = (size_t)row * a.D + 8 * c;
+                float2 dv[4], d[4];
+                if (RES != RES_NONE && a.dr_out) rd[v].get(d);
+                else d[0] = d[1] = d[2] = d[3] = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dv[e] = fma2(splat2(rstd), fma2(n[v][e], splat2(m), dn[v][e]), d[e]);
+                Oct<T> ox;
+                ox.set(dv);
+                ox.store(static_cast<T*>(a.dx) + at);
+                if (RES != RES_NONE && a.dr) {
+                    Oct<R> orr;
+                    orr.set(dv);
+                    orr.store(static_cast<R*>(a.dr) + at);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int c = lane + v * TPR;
+        if (c < nv) {
+            Oct<float> o;
+            o.set(dw[v]);
+            o.store(a.part_w + (size_t)group * a.D + 8 * c);
+        }
+    }
+}
+
+// the shares of dw added up in a fixed order: 32 columns per block, eight threads to a column
+__global__ void __launch_bounds__(256) kda_add_rms_norm_sum_kernel(const float* part, float* dw, int D, int rows) {
+    __shared__ float s[8][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), k0 = threadIdx.x >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    float sum = 0.f;
+    if (col < D) {
+#pragma unroll 8
+        for (int k = k0; k < rows; k += 8) sum += part[(size_t)k * D + col];
+    }
+    s[k0][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (k0 == 0 && col < D) {
+#pragma unroll
+        for (int k = 1; k < 8; ++k) sum += s[k][threadIdx.x];
+        dw[col] = sum;
+    }
+}
+
+// Threads and pieces for a row: a warp up to 1024 columns, two pieces per thread above that. Where rows are few, one piece per thread
+// (forward): a row's latency is then the call's.
+struct NormShape { int tpr, vpt; };
+static NormShape norm_shape(int D, long long R, bool backward) {
+    const int nv = D / 8;
+    if (nv <= 32) return {32, 1};
+    if (nv <= 64) return {32, 2};
+    if (nv <= 128) return {32, 4};
+    if (nv <= 512 && R <= 2LL * sm_count() && !backward) return {512, 1};
+    if (nv <= 256) return {128, 2};
+    if (nv <= 512) return {256, 2};
+    if (nv <= 1024) return {512, 2};
+    return {512, 4};
+}
+// f<TPR, VPT>() for a shape
+#define KDA_NORM_SHAPES(s, KERNEL)                                                                                              \
+    ((s).tpr == 32 ? ((s).vpt == 1 ? KERNEL(32, 1) : (s).vpt == 2 ? KERNEL(32, 2) : KERNEL(32, 4))                                  \
+     : (s).tpr == 128 ? KERNEL(128, 2) : (s).tpr == 256 ? KERNEL(256, 2)                                                          \
+     : (s).vpt == 1 ? KERNEL(512, 1) : (s).vpt == 2 ? KERNEL(512, 2) : KERNEL(512, 4))
+
+template <typename T, int RES, bool FP8>
+static int launch_norm_fwd(const AddNormArgs& a, cudaStream_t stream) {
+    const NormShape s = norm_shape(a.D, a.R, false);
+#define KDA_NORM_FWD(TPR, VPT) kda_add_rms_norm_fwd_kernel<T, RES, FP8, TPR, VPT>
+    void (*kernel)(const AddNormArgs) = KDA_NORM_SHAPES(s, KDA_NORM_FWD);
+#undef KDA_NORM_FWD
+    const int threads = norm_threads(s.tpr), groups = threads / s.tpr;
+    const long long want = (a.R + groups - 1) / groups, cap = sm_count() * (2048LL / threads);
+    return (int)launch_early(kernel, dim3((unsigned)(want < cap ? want : cap)), threads, 0, stream, a);
+}
+static long long norm_bwd_blocks(int D, long long R, NormShape s) {
+    const int groups = norm_threads(s.tpr) / s.tpr;
+    const long long want = (R + groups - 1) / groups, cap = sm_count() * (s.tpr == 512 ? 1LL : s.tpr == 256 ? 2LL : 4LL);
+    return want < cap ? want : cap;
+}
+template <typename T, int RES>
+static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
+    const NormShape s = norm_shape(a.D, a.R, true);
+#define KDA_NORM_BWD(TPR, VPT) kda_add_rms_norm_bwd_kernel<T, RES, TPR, VPT>
+    void (*kernel)(const AddNormArgs) = KDA_NORM_SHAPES(s, KDA_NORM_BWD);
+#undef KDA_NORM_BWD
+    const int threads = norm_threads(s.tpr), groups = threads / s.tpr;
+    const long long blocks = norm_bwd_blocks(a.D, a.R, s);
+    if (const cudaError_t e = launch_early(kernel, dim3((unsigned)blocks), threads, 0, stream, a); e != cudaSuccess) return (int)e;
+    return (int)launch_early(kda_add_rms_norm_sum_kernel, dim3((a.D + 31) / 32), 256, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)(blocks * groups));
+}
+
+}  // namespace kda
+
+// rows of `part_w` that the backward pass writes
+extern "C" int kda_add_rms_norm_shares(int D, long long R) {
+    using namespace kda;
+    const NormShape s = norm_shape(D, R, true);
+    return (int)norm_bwd_blocks(D, R, s) * (norm_threads(s.tpr) / s.tpr);
+}
+
+extern "C" int kda_launch_add_rms_norm(const kda::AddNormArgs* a, int backward, cudaStream_t stream) {
+    using namespace kda;
+    using bf16 = __nv_bfloat16;
+    if (a->R <= 0) return 0;
+    if (a->D % 8 || a->D > 16384) return -1;
+#define KDA_NORM(T, RES) return backward ? launch_norm_bwd<T, RES>(*a, stream) : a->fp8 ? launch_norm_fwd<T, RES, true>(*a, stream) : launch_norm_fwd<T, RES, false>(*a, stream)
+    if (!a->fp32) {
+        if (a->res == RES_NONE) KDA_NORM(bf16, RES_NONE);
+        if (a->res == RES_BF16) KDA_NORM(bf16, RES_BF16);
+        KDA_NORM(bf16, RES_FP32);
+    }
+    if (a->res == RES_NONE) KDA_NORM(float, RES_NONE);
+    if (a->res == RES_FP32) KDA_NORM(float, RES_FP32);
+#undef KDA_NORM
+    return -1;
+}

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/cula_kda.h"
+
 namespace kda {
 
 enum GateMode : int {
@@ -159,6 +161,12 @@ struct ConvArgs {
     const int* chunk_indices;     // [NT][2] or null
     int T, D, W, silu;
 };
+
+// the operators of a selective state space block take their arguments as the C structures of the library's header
+using SelScanArgs = ::cula_kda_selective_scan_args;
+using SelStepArgs = ::cula_kda_selective_step_args;
+using ConvStepArgs = ::cula_kda_conv_step_args;
+using AddNormArgs = ::cula_kda_add_rms_norm_args;
 
 // gated RMS norm (forward and backward)
 struct NormArgs {

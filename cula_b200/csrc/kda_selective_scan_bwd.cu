@@ -1,0 +1,469 @@
+// Selective scan, backward (definition and layout: selective_scan.cuh). With g_t the gradient of h_t,
+//     g_t = dy_t C_t + a_{t+1} g_{t+1},     a_t = exp(dt_t A),     dy_t = dout_t silu(z_t)
+//     dC_t = sum_d dy_t h_t            dB_t = sum_d g_t dt_t x_t         dA = sum_t w_t dt_t,   w_t = a_t g_t h_{t-1}
+//     dx_t = dt_t sum_n g_t B_t + skip dy_t                              ddt_t = x_t sum_n g_t B_t + sum_n w_t A
+//     dz_t = dout_t y_t silu'(z_t)     dskip = sum_t dy_t x_t            dh0 = a_1 g_1
+// One CTA walks a segment of a sequence backwards for a tile of channels. The states between are made again, eight tokens at a time, from
+// those that the forward pass kept, and stay in registers together with the a_t until the way back has used them. Sums over states go over
+// the lanes of a channel, sums over channels over the lanes of a state and the warps; the tiles' shares of dB and dC and the CTAs' shares
+// of dA, dskip and dbias are added up by a second kernel in a fixed order, so that every gradient is the same from run to run.
+#include "selective_scan.cuh"
+
+namespace kda {
+
+template <int SL, typename T>
+struct SelBwdSmem {
+    using G = SelShape<SL>;
+    static constexpr int Q = SelVec<T>::Q;
+    float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
+    float2 dy[2][G::LC][G::CH / 2];
+    float4 b[2][G::LC][SL], c[2][G::LC][SL];
+    float2 sums[2][G::LC][G::CH];                                    // per channel: sum_n g B, sum_n w A (log2 units)
+    float bc[2][SEL_WARPS][G::LC][2 * G::SP];                        // per warp: dB, dC
+    uint4 raw[3][4][Q][G::ITEMS];                                 // x, dt, z, dout rows as they are
+    float4 acc[4][SEL_THREADS];                                      // a thread's sums for dskip and dbias (8 channels each)
+};
+
+// STATE_ONLY: what each segment adds to the gradient of the state that leaves it, and the sum of its steps
+template <int SL, typename T, bool STATE_ONLY>
+__global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective_scan_bwd_kernel(const SelScanArgs a, const int tiles_per_group, const long long items) {
+    using G = SelShape<SL>;
+    using V = SelVec<T>;
+    constexpr int LC = G::LC, CH = G::CH, CL = G::CL, SP = G::SP, Q = V::Q, KEEP = SEL_KEEP;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    SelBwdSmem<SL, T>& sm = *reinterpret_cast<SelBwdSmem<SL, T>*>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tiles = tiles_per_group * a.G, tile = blockIdx.x % tiles, row = blockIdx.x / tiles;
+    const int group = tile / tiles_per_group, per_group = a.D / a.G;
+    const int d0 = group * per_group + (tile % tiles_per_group) * CH, d_end = (group + 1) * per_group;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int cl = lane & (CL - 1), s = lane / CL, n0 = 4 * s, pair = warp * CL + cl, dc = d0 + 2 * pair;
+    const bool own = dc < d_end;
+    float2 A2[2][2], dA[2][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        dA[c][0] = dA[c][1] = A2[c][0] = A2[c][1] = make_float2(0.f, 0.f);
+        if (own) {
+            sel_load4(a.A + (size_t)(dc + c) * a.S, n0, a.S, A2[c]);
+            A2[c][0] = mul2(A2[c][0], splat2(RCP_LN2));
+            A2[c][1] = mul2(A2[c][1], splat2(RCP_LN2));
+        }
+    }
+    const int tt = tid / G::VECS, vec = tid % G::VECS, dv = d0 + 8 * vec;
+    const bool item = tid < G::ITEMS && dv < d_end, gate = a.z != nullptr;
+    if constexpr (!STATE_ONLY) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+
+    for (long long i = row; i < items; i += a.cta_rows) {
+        SelItem it;
+        if (!sel_item(a, i, it)) continue;
+        if (STATE_ONLY && it.seg == 0) continue;                     // nothing comes before it
+        const int batch = a.cu_seqlens ? 0 : it.seq;
+        const long long first = a.cu_seqlens ? it.row0 : 0;
+        const T* xp = static_cast<const T*>(a.x) + batch * a.x_seq + first * a.x_row + dv;
+        const T* dtp = static_cast<const T*>(a.dt) + batch * a.dt_seq + first * a.dt_row + dv;
+        const T* zp = static_cast<const T*>(a.z) + batch * a.z_seq + first * a.z_row + dv;
+        const T* dop = static_cast<const T*>(a.dy) + (size_t)it.row0 * a.D + dv;
+        const T* bp = static_cast<const T*>(a.Bm) + batch * a.b_seq + first * a.b_row + group * a.S;
+        const T* cp = static_cast<const T*>(a.Cm) + batch * a.c_seq + first * a.c_row + group * a.S;
+        const int n_tiles = (it.t1 - it.t0 + LC - 1) / LC;
+
+        float2 gh[2][2];                                             // a_{t+1} g_{t+1}: the gradient of h_t through what comes after
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            gh[c][0] = gh[c][1] = make_float2(0.f, 0.f);
+            if (!STATE_ONLY && own && a.dhT) sel_load4(a.dhT + ((size_t)it.seq * a.D + dc + c) * a.S, n0, a.S, gh[c]);
+        }
+        if constexpr (!STATE_ONLY) {
+            if (own) {                                               // the segments after this one
+#pragma unroll 2
+                for (int q = it.segs - 1; q > it.seg; --q) {
+                    const size_t at = (size_t)(it.slot0 + q) * a.D + dc;
+                    const float2 sum = *reinterpret_cast<const float2*>(a.seg_dt + at);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float4 add = *reinterpret_cast<const float4*>(a.seg_state + (at + c) * SP + n0);
+                        const float2 d = splat2(c ? sum.y : sum.x);
+                        gh[c][0] = fma2(ex2_2(mul2(d, A2[c][0])), gh[c][0], make_float2(add.x, add.y));
+                        gh[c][1] = fma2(ex2_2(mul2(d, A2[c][1])), gh[c][1], make_float2(add.z, add.w));
+                    }
+                }
+            }
+        }
+
+        // tiles are taken from the last to the first; the j-th taken is tile n_tiles - 1 - j
+        auto fetch = [&](int j) {
+            const int t = it.t0 + (n_tiles - 1 - j) * LC + tt;
+            if (item && j < n_tiles && t < it.t1) {
+                uint4(*to)[Q][G::ITEMS] = sm.raw[j % 3];
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    sel_copy16(&to[0][q][tid], xp + (long long)t * a.x_row + q * (8 / Q));
+                    sel_copy16(&to[1][q][tid], dtp + (long long)t * a.dt_row + q * (8 / Q));
+                    if (gate) sel_copy16(&to[2][q][tid], zp + (long long)t * a.z_row + q * (8 / Q));
+                    sel_copy16(&to[3][q][tid], dop + (size_t)t * a.D + q * (8 / Q));
+                }
+            }
+            sel_commit();
+        };
+        float4 rb[G::UB], rc[G::UB];
+        auto fetch_bc = [&](int j) {
+#pragma unroll
+            for (int u = 0; u < G::UB; ++u) {
+                const int i = u * SEL_THREADS + tid, t = it.t0 + (n_tiles - 1 - j) * LC + i / SL;
+                const bool ok = i < G::UNITS && j < n_tiles && t < it.t1;
+                if (!STATE_ONLY) rb[u] = ok ? sel_four(bp + (long long)t * a.b_row, 4 * (i % SL), a.S, a.vec_bc) : make_float4(0.f, 0.f, 0.f, 0.f);
+                rc[u] = ok ? sel_four(cp + (long long)t * a.c_row, 4 * (i % SL), a.S, a.vec_bc) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        auto stage = [&](int j) {
+            const int buf = j & 1;
+            if (tid < G::ITEMS) {                                    // zeros for channels past the tile: they add nothing to dB and dC
+                const bool live = item && it.t0 + (n_tiles - 1 - j) * LC + tt < it.t1;
+                float2 x[4], d[4], z[4], o[4];
+                if (live) {
+                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j % 3];
+                    V::unpack(&from[0][0][tid], G::ITEMS, x);
+                    V::unpack(&from[1][0][tid], G::ITEMS, d);
+                    if (gate) V::unpack(&from[2][0][tid], G::ITEMS, z);
+                    V::unpack(&from[3][0][tid], G::ITEMS, o);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float2 step = make_float2(0.f, 0.f), prod = step, dy = step;
+                    if (live) {
+                        step = a.dt_bias ? add2(d[e], *reinterpret_cast<const float2*>(a.dt_bias + dv + 2 * e)) : d[e];
+                        if (a.softplus) step = softplus2(step);
+                        prod = mul2(step, x[e]);
+                        dy = gate ? mul2(mul2(o[e], z[e]), sel_sigmoid2(z[e])) : o[e];
+                    }
+                    sm.dx[buf][tt][vec * 4 + e] = make_float4(step.x, step.y, prod.x, prod.y);
+                    sm.dy[buf][tt][vec * 4 + e] = dy;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < G::UB; ++u) {
+                const int i = u * SEL_THREADS + tid;
+                if (i < G::UNITS) {
+                    if (!STATE_ONLY) sm.b[buf][i / SL][i % SL] = rb[u];
+                    sm.c[buf][i / SL][i % SL] = rc[u];
+                }
+            }
+        };
+
+        float2 sum_dt = make_float2(0.f, 0.f);
+        if (n_tiles > 0) {
+            fetch(0);
+            fetch(1);
+            fetch_bc(0);
+            sel_wait<1>();
+            stage(0);
+            __syncthreads();
+        }
+        for (int j = 0; j < n_tiles; ++j) {
+            const int buf = j & 1, tile_t0 = it.t0 + (n_tiles - 1 - j) * LC;
+            fetch(j + 2);
+            fetch_bc(j + 1);
+            if constexpr (STATE_ONLY) {
+#pragma unroll 8
+                for (int u = LC - 1; u >= 0; --u) {
+                    const float4 dx = sm.dx[buf][u][pair], cc = sm.c[buf][u][s];
+                    const float2 dy = sm.dy[buf][u][pair];
+                    sum_dt = add2(sum_dt, make_float2(dx.x, dx.y));
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float2 d = splat2(c ? dx.y : dx.x), o = splat2(c ? dy.y : dy.x);
+                        gh[c][0] = mul2(ex2_2(mul2(d, A2[c][0])), fma2(o, make_float2(cc.x, cc.y), gh[c][0]));
+                        gh[c][1] = mul2(ex2_2(mul2(d, A2[c][1])), fma2(o, make_float2(cc.z, cc.w), gh[c][1]));
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int sub = LC / KEEP - 1; sub >= 0; --sub) {
+                    const int tb = sub * KEEP;
+                    if (tile_t0 + tb >= it.t1) continue;             // past the end: nothing in it
+                    float2 st[KEEP + 1][2][2], av[KEEP][2][2];       // states before and after each token; a_t
+                    {
+                        const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + (tile_t0 + tb) / KEEP) * a.D + dc) * SP + n0;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float4 r = own ? *reinterpret_cast<const float4*>(from + c * SP) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            st[0][c][0] = make_float2(r.x, r.y);
+                            st[0][c][1] = make_float2(r.z, r.w);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < KEEP; ++u) {
+                        const float4 dx = sm.dx[buf][tb + u][pair], b = sm.b[buf][tb + u][s];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float2 d = splat2(c ? dx.y : dx.x), p = splat2(c ? dx.w : dx.z);
+                            av[u][c][0] = ex2_2(mul2(d, A2[c][0]));
+                            av[u][c][1] = ex2_2(mul2(d, A2[c][1]));
+                            st[u + 1][c][0] = fma2(p, make_float2(b.x, b.y), mul2(av[u][c][0], st[u][c][0]));
+                            st[u + 1][c][1] = fma2(p, make_float2(b.z, b.w), mul2(av[u][c][1], st[u][c][1]));
+                        }
+                    }
+                    float2 dA8[2][2];                                // eight terms are added up first
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) dA8[c][0] = dA8[c][1] = make_float2(0.f, 0.f);
+                    constexpr int TB = SL > 4 ? SL / 4 : 1;          // tokens whose sums over states are added up together
+                    float v[4 * TB];
+#pragma unroll
+                    for (int u = KEEP - 1; u >= 0; --u) {
+                        const float4 dx = sm.dx[buf][tb + u][pair], b = sm.b[buf][tb + u][s], cc = sm.c[buf][tb + u][s];
+                        const float2 dy = sm.dy[buf][tb + u][pair];
+                        float2 dB0 = make_float2(0.f, 0.f), dB1 = dB0, dC0 = dB0, dC1 = dB0;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float2 d = splat2(c ? dx.y : dx.x), p = splat2(c ? dx.w : dx.z), o = splat2(c ? dy.y : dy.x);
+                            const float2 g0 = fma2(o, make_float2(cc.x, cc.y), gh[c][0]), g1 = fma2(o, make_float2(cc.z, cc.w), gh[c][1]);
+                            dC0 = fma2(o, st[u + 1][c][0], dC0);
+                            dC1 = fma2(o, st[u + 1][c][1], dC1);
+                            dB0 = fma2(g0, p, dB0);
+                            dB1 = fma2(g1, p, dB1);
+                            const float2 s1 = fma2(g1, make_float2(b.z, b.w), mul2(g0, make_float2(b.x, b.y)));
+                            gh[c][0] = mul2(av[u][c][0], g0);
+                            gh[c][1] = mul2(av[u][c][1], g1);
+                            const float2 w0 = mul2(gh[c][0], st[u][c][0]), w1 = mul2(gh[c][1], st[u][c][1]);
+                            const float2 s2 = fma2(w1, A2[c][1], mul2(w0, A2[c][0]));
+                            dA8[c][0] = fma2(w0, d, dA8[c][0]);
+                            dA8[c][1] = fma2(w1, d, dA8[c][1]);
+                            v[4 * (u % TB) + 2 * c] = s1.x + s1.y;
+                            v[4 * (u % TB) + 2 * c + 1] = s2.x + s2.y;
+                        }
+                        if (u % TB == 0) {                           // values: (token, channel, which sum)
+                            float r[4 * TB];
+#pragma unroll
+                            for (int k = 0; k < 4 * TB; ++k) r[k] = v[k];
+                            sel_reduce<4 * TB, SL>(r, lane, CL);
+                            constexpr int LEFT = 4 * TB / SL;        // 1, or 2 where two lanes share four values
+                            const int at = s * LEFT;
+#pragma unroll
+                            for (int k = 0; k < LEFT; ++k) {
+                                const int id = at + k, tok = id / 4, ch = (id >> 1) & 1, which = id & 1;
+                                reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][2 * pair + ch])[which] = r[k];
+                            }
+                        }
+                        float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
+                        sel_reduce<8, CL>(r, lane, 1);
+                        if constexpr (CL >= 8) {
+                            constexpr int REP = CL / 8;              // lanes left with the same value
+                            if (REP == 1 || cl % REP == 0) {
+                                const int id = cl / REP;
+                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
+                            }
+                        } else {
+                            constexpr int LEFT = 8 / CL;
+#pragma unroll
+                            for (int k = 0; k < LEFT; ++k) {
+                                const int id = cl * LEFT + k;
+                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        dA[c][0] = add2(dA[c][0], dA8[c][0]);
+                        dA[c][1] = add2(dA[c][1], dA8[c][1]);
+                    }
+                }
+            }
+            if (j + 1 < n_tiles) {
+                sel_wait<1>();
+                stage(j + 1);
+            }
+            __syncthreads();
+            if constexpr (!STATE_ONLY) {
+                const int t = tile_t0 + tt;
+                if (item && t < it.t1) {
+                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j % 3];
+                    const size_t at = (size_t)(it.row0 + t) * a.D + dv;
+                    float2 x[4], d[4], o[4];
+                    V::unpack(&from[0][0][tid], G::ITEMS, x);
+                    V::unpack(&from[1][0][tid], G::ITEMS, d);
+                    float4 acc[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = sm.acc[e][tid];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 step = sm.dx[buf][tt][vec * 4 + e];
+                        const float2 dy = sm.dy[buf][tt][vec * 4 + e];
+                        const float4 sums = *reinterpret_cast<const float4*>(&sm.sums[buf][tt][8 * vec + 2 * e]);
+                        const float2 gB = make_float2(sums.x, sums.z), wA = make_float2(sums.y, sums.w);
+                        float2 dd = fma2(x[e], gB, mul2(wA, splat2(0.6931471805599453f)));          // A is held times log2(e)
+                        if (a.softplus) {
+                            const float2 raw = a.dt_bias ? add2(d[e], *reinterpret_cast<const float2*>(a.dt_bias + dv + 2 * e)) : d[e];
+                            dd = mul2(dd, sel_sigmoid2(raw));
+                        }
+                        const float2 skip = a.skip ? *reinterpret_cast<const float2*>(a.skip + dv + 2 * e) : make_float2(0.f, 0.f);
+                        const float2 dxv = fma2(make_float2(step.x, step.y), gB, mul2(skip, dy));
+                        const float2 ds = mul2(dy, x[e]);
+                        float4& as = acc[e / 2];
+                        float4& ab = acc[2 + e / 2];
+                        if (e & 1) { as.z += ds.x; as.w += ds.y; ab.z += dd.x; ab.w += dd.y; }
+                        else { as.x += ds.x; as.y += ds.y; ab.x += dd.x; ab.y += dd.y; }
+                        d[e] = dd;
+                        x[e] = dxv;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sm.acc[e][tid] = acc[e];
+                    V::store(static_cast<T*>(a.dx) + at, x);
+                    V::store(static_cast<T*>(a.ddt) + at, d);
+                    if (gate) {
+                        float2 z[4];
+                        V::unpack(&from[2][0][tid], G::ITEMS, z);
+                        V::unpack(&from[3][0][tid], G::ITEMS, o);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 y = *reinterpret_cast<const float2*>(a.y_pre + at + 2 * e), sg = sel_sigmoid2(z[e]);
+                            // silu' = s (1 + z (1 - s))
+                            o[e] = mul2(mul2(o[e], y), mul2(sg, fma2(z[e], fma2(sg, splat2(-1.f), splat2(1.f)), splat2(1.f))));
+                        }
+                        V::store(static_cast<T*>(a.dz) + at, o);
+                    }
+                }
+                // this tile of channels' share of dB and dC
+                for (int i = tid; i < LC * SP / 2; i += SEL_THREADS) {
+                    const int u = i / (SP / 2), n = 4 * (i % (SP / 2));
+                    if (tile_t0 + u < it.t1) {
+                        float4 sum = *reinterpret_cast<const float4*>(&sm.bc[buf][0][u][n]);
+#pragma unroll
+                        for (int w = 1; w < SEL_WARPS; ++w) {
+                            const float4 r = *reinterpret_cast<const float4*>(&sm.bc[buf][w][u][n]);
+                            sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
+                        }
+                        const size_t at = (((size_t)(tile % tiles_per_group) * a.rows + it.row0 + tile_t0 + u) * a.G + group) * (2 * SP) + n;
+                        *reinterpret_cast<float4*>(a.part_bc + at) = sum;
+                    }
+                }
+            }
+        }
+        sel_wait<0>();
+        __syncthreads();                                             // the next item stages into the same buffers
+        if (own) {
+            if constexpr (STATE_ONLY) {
+                const size_t at = (size_t)(it.slot0 + it.seg) * a.D + dc;
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    *reinterpret_cast<float4*>(a.seg_state + (at + c) * SP + n0) = make_float4(gh[c][0].x, gh[c][0].y, gh[c][1].x, gh[c][1].y);
+                if (s == 0) *reinterpret_cast<float2*>(a.seg_dt + at) = sum_dt;
+            } else if (a.dh0 && it.seg == 0) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) sel_store4(a.dh0 + ((size_t)it.seq * a.D + dc + c) * a.S, n0, a.S, gh[c]);
+            }
+        }
+    }
+    if constexpr (!STATE_ONLY) {
+        if (own) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                *reinterpret_cast<float4*>(a.part_A + ((size_t)row * a.D + dc + c) * SP + n0) = make_float4(dA[c][0].x, dA[c][0].y, dA[c][1].x, dA[c][1].y);
+        }
+        __syncthreads();
+        // dskip and dbias: the threads that stood at the same channels, in order
+        for (int i = tid; i < 4 * G::VECS; i += SEL_THREADS) {
+            const int v = i % G::VECS, e = i / G::VECS;
+            if (d0 + 8 * v < d_end) {
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = v; k < G::ITEMS; k += G::VECS) {
+                    const float4 r = sm.acc[e][k];
+                    sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
+                }
+                float* to = e < 2 ? a.part_skip : a.part_bias;
+                if (to) *reinterpret_cast<float4*>(to + (size_t)row * a.D + d0 + 8 * v + 4 * (e & 1)) = sum;
+            }
+        }
+    }
+}
+
+// ---- the shares added up: dB and dC (one thread per token row, group and four states), then dA, dskip, dbias (one per value) ----
+template <typename T>
+__global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blockIdx.x < bc_blocks) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x, quads = SP / 2, rg = i / quads;
+        if (rg >= a.rows * a.G) return;
+        const int q = (int)(i - rg * quads), isC = q >= SP / 4, n = 4 * (q % (SP / 4));
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!a.cu_seqlens || rg / a.G < a.total_tokens) {            // rows past the packed tokens have zero gradients
+#pragma unroll 8
+            for (int k = 0; k < tiles_per_group; ++k) {
+                const float4 r = *reinterpret_cast<const float4*>(a.part_bc + ((size_t)k * a.rows * a.G + rg) * (2 * SP) + 4 * q);
+                sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
+            }
+        }
+        T* to = static_cast<T*>(isC ? a.dCm : a.dBm) + rg * a.S;
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (n + k < a.S) {
+                if constexpr (sizeof(T) == 4) to[n + k] = f[k];
+                else to[n + k] = __float2bfloat16_rn(f[k]);
+            }
+        }
+    } else {
+        const long long i = (long long)(blockIdx.x - bc_blocks) * 256 + threadIdx.x, nA = (long long)a.D * SP;
+        const float* from = i < nA ? a.part_A + i : i < nA + a.D ? a.part_skip + (i - nA) : a.part_bias + (i - nA - a.D);
+        const long long stride = i < nA ? nA : a.D;
+        if (i >= nA + 2LL * a.D) return;
+        if ((i >= nA && i < nA + a.D && !a.dskip) || (i >= nA + a.D && !a.dbias)) return;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < a.cta_rows; ++k) sum += from[k * stride];
+        if (i < nA) {
+            const int n = (int)(i % SP);
+            if (n < a.S) a.dA[i / SP * a.S + n] = sum;
+        } else if (i < nA + a.D) a.dskip[i - nA] = sum;
+        else a.dbias[i - nA - a.D] = sum;
+    }
+}
+
+template <int SL, typename T>
+static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
+    using G = SelShape<SL>;
+    const int tpg = (a.D / a.G + G::CH - 1) / G::CH;
+    const long long items = sel_items(a);
+    const long long blocks = (long long)a.cta_rows * tpg * a.G;
+    if (blocks <= 0 || blocks > 0x7fffffffLL) return -1;
+    static_assert(sizeof(SelBwdSmem<SL, T>) <= 227 * 1024, "");
+    constexpr int smem = sizeof(SelBwdSmem<SL, T>);
+    static std::atomic<unsigned long long> done[2];
+    if (a.seg_chunks) {
+        if (const cudaError_t e = allow_smem(kda_selective_scan_bwd_kernel<SL, T, true>, smem, done[1]); e != cudaSuccess) return (int)launched(e);
+        if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, true>, dim3((unsigned)blocks), SEL_THREADS, smem, stream, a, tpg, items);
+            e != cudaSuccess)
+            return (int)e;
+    }
+    if (const cudaError_t e = allow_smem(kda_selective_scan_bwd_kernel<SL, T, false>, smem, done[0]); e != cudaSuccess) return (int)launched(e);
+    if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_THREADS, smem, stream, a, tpg, items);
+        e != cudaSuccess)
+        return (int)e;
+    const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 255) / 256, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
+    if (bc_blocks + rest > 0x7fffffffLL) return -1;
+    return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks);
+}
+
+}  // namespace kda
+
+// what a caller has to provide for part_bc: channel tiles per group
+extern "C" int kda_selective_scan_tiles(int D, int groups, int state_lanes) {
+    const int ch = 256 / state_lanes;
+    return (D / groups + ch - 1) / ch;
+}
+
+extern "C" int kda_launch_selective_scan_bwd(const kda::SelScanArgs* a, int state_lanes, cudaStream_t stream) {
+    using namespace kda;
+    switch (state_lanes) {
+        case 2: return a->fp32 ? launch_sel_bwd<2, float>(*a, stream) : launch_sel_bwd<2, __nv_bfloat16>(*a, stream);
+        case 4: return a->fp32 ? launch_sel_bwd<4, float>(*a, stream) : launch_sel_bwd<4, __nv_bfloat16>(*a, stream);
+        case 8: return a->fp32 ? launch_sel_bwd<8, float>(*a, stream) : launch_sel_bwd<8, __nv_bfloat16>(*a, stream);
+        case 16: return a->fp32 ? launch_sel_bwd<16, float>(*a, stream) : launch_sel_bwd<16, __nv_bfloat16>(*a, stream);
+    }
+    return -1;
+}

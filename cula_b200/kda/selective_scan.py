@@ -1,0 +1,39 @@
+"""The selective state space recurrence: ``selective_scan`` over whole sequences, with gradients, and ``selective_scan_update`` for one
+token of each sequence against a pool of states. Hand-written sm_100a kernels (csrc/kda_selective_scan_fwd.cu, _bwd.cu,
+kda_selective_step.cu); checks, autograd and launches in the host extension (csrc/host/host_ssm.cpp). No Triton, no fallback."""
+from __future__ import annotations
+
+import torch
+
+from .. import _native
+from ..utils import get_varlen_tables
+
+
+@torch.compiler.disable
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, initial_state=None, output_final_state=False,
+                   cu_seqlens=None, cu_seqlens_cpu=None):
+    """Per channel ``d`` and state ``n``, with ``step = softplus(dt + dt_bias)`` (or ``dt + dt_bias``)::
+
+        h_t = exp(step_t * A[d, n]) * h_{t-1} + step_t * x_t * B_t[n]
+        y_t = (sum_n C_t[n] * h_t[n] + D * x_t) * silu(z_t)
+
+    x, dt, z: ``[B, T, D]`` bf16 or fp32 (``B == 1`` with ``cu_seqlens``); A: ``[D, S]``, ``S <= 64``; B, C: ``[B, T, S]``, or
+    ``[B, T, G, S]`` for groups of ``D / G`` channels (a multiple of 8); D, dt_bias: ``[D]`` or None; z None: no gate. Activations
+    have one type; views of a projection's output are read in place. initial_state: ``[N, D, S]`` fp32 or None for zeros, one per
+    sequence; with ``output_final_state`` the states after the last tokens are returned, of a sequence without tokens the one before.
+    Rows of a packed batch past its last token have zero outputs and gradients. States and sums are fp32.
+
+    Returns ``(y, final_state)``, y in the type of x. Gradients flow from both to every tensor argument and are the same from run to
+    run; a forward call that gradients will be asked of keeps the states before every eighth token (fp32)."""
+    tab = None if cu_seqlens is None else get_varlen_tables(cu_seqlens, cu_seqlens_cpu).native
+    return _native.host().selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, tab)
+
+
+def selective_scan_update(x, dt, A, B, C, state, state_indices=None, D=None, z=None, dt_bias=None, dt_softplus=False, out=None):
+    """One token of ``selective_scan`` for each of ``N`` sequences, as a decode step.
+
+    x, dt, z: ``[N, D]`` (or ``[N, 1, D]``); B, C: ``[N, S]`` or ``[N, G, S]`` (with x's token axis, if it has one); state:
+    ``[pool, D, S]`` fp32, contiguous, updated in place. state_indices: ``[N]`` int32 slots, negative = skip the sequence (zero output,
+    no access to the pool), or None for slot = sequence; a slot may be named once in a call. A slot past the pool is skipped too and
+    reported by ``check_status``. Returns ``y`` shaped like x (``out`` if given). No gradients."""
+    return _native.host().selective_scan_update(x, dt, A, B, C, state, state_indices, D, z, dt_bias, dt_softplus, out)

@@ -67,6 +67,7 @@ class VarlenTables:
         host[2 * NT + 2 * n + 2:] = np.argsort(-lens, kind="stable")
         device = torch.from_numpy(host).to(cu_seqlens.device)
         self.n_seqs, self.num_chunks, self.total_tokens = n, NT, int(bounds[-1])
+        self.longest = int(n_chunks.max()) if n else 0               # chunks of the longest sequence
         self.chunk_indices = device[:2 * NT].view(NT, 2)
         self.chunk_offsets, self.cu_seqlens, self.seq_order = device[2 * NT:].split([n + 1, n + 1, n])
         self.seqlens_cpu = cpu
@@ -77,7 +78,7 @@ class VarlenTables:
         """The same tables as the host extension takes them."""
         if self._native is None:
             self._native = _native.host().Tables(self.cu_seqlens, self.chunk_indices, self.chunk_offsets, self.seq_order,
-                                                 self.n_seqs, self.num_chunks, self.total_tokens)
+                                                 self.n_seqs, self.num_chunks, self.total_tokens, self.longest)
         return self._native
 
     @property

@@ -305,6 +305,118 @@ int cula_kda_rms_norm_gated_bwd(const void* d_x, const void* d_g, const float* d
                                 const void* d_dy, void* d_dx, void* d_dg, float* d_dw, long long R, int D,
                                 int use_swish, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators of a selective state space block. Their arguments are structures, passed by address and read during the call; pointers are
+ * device pointers, members that an entry point does not use may hold anything. Activations are bf16, or fp32 with `fp32` set, all of one type.
+ *
+ * Selective scan over whole sequences, per channel d (group g = d / (D / G)) and state n:
+ *     step_t = softplus(dt_t + dt_bias) (or without softplus),   h_t = exp(step_t A) h_{t-1} + step_t x_t B_t
+ *     y_t = (sum_n C_t[n] h_t[n] + skip x_t) silu(z_t)
+ * Rows of x, dt, z, B and C may be strided (row: elements from a token to the next, seq: from a sequence of a fixed-length batch to the
+ * next); their innermost dimensions are contiguous, rows of x, dt and z are 16-byte aligned, D / G is a multiple of 8, S <= 64. Everything
+ * else is contiguous. A sequence is walked in one piece, or (seg_chunks) in segments of that many 64-token chunks side by side, for which a
+ * launch before finds what each adds to the state.
+ * SP below is the smallest of 8, 16, 32 and 64 that holds S.
+ * ------------------------------------------------------------------------------------------------------------ */
+typedef struct cula_kda_selective_scan_args {
+    const void *x, *dt, *z;       /* [B, T, D]; z NULL: no gate */
+    const void *Bm, *Cm;          /* [B, T, G, S] */
+    long long x_row, dt_row, z_row, b_row, c_row;
+    long long x_seq, dt_seq, z_seq, b_seq, c_seq;
+    const float* A;               /* [D, S] */
+    const float* skip;            /* [D] or NULL */
+    const float* dt_bias;         /* [D] or NULL */
+    const float* h0;              /* [N, D, S] or NULL */
+    void* y;                      /* [B*T, D]                                                                  (forward) */
+    float* hT;                    /* [N, D, S] or NULL                                                         (forward) */
+    float* states;                /* [num_chunks * 8, D, SP]: the state before every eighth token; forward: NULL unless a backward pass follows */
+    float* y_pre;                 /* [B*T, D]: y before the gate, with z and `states` */
+    const void* dy;               /* [B*T, D]                                                                  (backward from here) */
+    const float* dhT;             /* [N, D, S] or NULL */
+    void *dx, *ddt, *dz;          /* [B*T, D]; dz with z */
+    void *dBm, *dCm;              /* [B*T, G, S] */
+    float *dA, *dskip, *dbias;    /* [D, S], [D], [D]; dskip and dbias may be NULL */
+    float* dh0;                   /* [N, D, S] or NULL */
+    float* part_bc;               /* workspace [cula_kda_selective_scan_tiles(), B*T, G, 2, SP] */
+    float* part_A;                /* workspaces [cta_rows, D, SP], [cta_rows, D], [cta_rows, D] (the latter two with dskip, dbias) */
+    float *part_skip, *part_bias;
+    float* seg_state;             /* with seg_chunks, workspaces [segments, D, SP] and [segments, D]; segments = N ceil(chunks / seg_chunks), */
+    float* seg_dt;                /* or num_chunks / seg_chunks + N for a packed batch */
+    const int *cu_seqlens, *chunk_indices, *chunk_offsets, *seq_order;      /* packed batch (cula_kda_build_chunk_tables), or NULL */
+    long long rows;               /* B*T */
+    int T, D, S, G, n_seqs, num_chunks, total_tokens;       /* total_tokens: of a packed batch */
+    int seg_chunks;               /* 0: sequences are not cut */
+    int cta_rows;                 /* how many CTAs share the sequences (or segments) per tile of channels (backward) */
+    int softplus, fp32;
+    int vec_bc;                   /* rows of B and C begin where four states can be loaded at once */
+} cula_kda_selective_scan_args;
+int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* args, void* stream);
+int cula_kda_selective_scan_bwd(const cula_kda_selective_scan_args* args, void* stream);
+/* channel tiles of a group, the first dimension of part_bc */
+int cula_kda_selective_scan_tiles(int D, int G, int S);
+
+/* One token of that recurrence for each of `rows` sequences against a pool of states, updated in place. Negative slots skip a row (zero
+ * output); slots past the pool do so too and set *status to 2. A slot may appear once in a call. */
+typedef struct cula_kda_selective_step_args {
+    const void *x, *dt, *z;       /* [rows, D]; z NULL: no gate */
+    const void *Bm, *Cm;          /* [rows, G, S] */
+    const float* A;               /* [D, S] */
+    const float* skip;            /* [D] or NULL */
+    const float* dt_bias;         /* [D] or NULL */
+    float* state;                 /* [pool, D, S] */
+    const int* indices;           /* [rows], or NULL: slot = row */
+    void* y;                      /* [rows, D] */
+    long long x_row, dt_row, z_row, b_row, c_row;
+    int rows, D, S, G, pool, softplus, fp32;
+    int vec;                      /* rows of states, A, B and C can be read four states at a time */
+    int* status;
+} cula_kda_selective_step_args;
+int cula_kda_selective_step(const cula_kda_selective_step_args* args, void* stream);
+
+/* One token of the short convolution (W <= 4, D a multiple of 8) for each of `rows` sequences: the window of the last W inputs, newest
+ * last, as cula_kda_short_conv_fwd leaves it in d_cache_out, takes in x and is applied. Slots as above. */
+typedef struct cula_kda_conv_step_args {
+    const void* x;                /* [rows, D] bf16 */
+    const float* w;               /* [D, W] */
+    const float* bias;            /* [D] or NULL */
+    float* cache;                 /* [pool, D, W] */
+    const int* indices;           /* [rows], or NULL: slot = row */
+    void* y;                      /* [rows, D] bf16 */
+    long long x_row;
+    int rows, D, W, pool, silu;
+    int* status;
+} cula_kda_conv_step_args;
+int cula_kda_conv_step(const cula_kda_conv_step_args* args, void* stream);
+
+/* v = x + r in the type of the residual stream r (res: 0 none, 1 bf16, 2 fp32), y = v rsqrt(mean(v^2) + eps) w; with fp8, y is e4m3 and
+ * scale[row] or scale[row, column / group] = max(amax / 448, 2^-126). D a multiple of 8 up to 16384; group 32, 64, 128, 256 or 0.
+ * Backward: dx and (where its type differs) dr from dy and dr_out, dw by way of part_w. */
+typedef struct cula_kda_add_rms_norm_args {
+    const void* x;                /* [R, D] */
+    const void* r;                /* [R, D] or NULL */
+    const float* w;               /* [D] */
+    void* y;                      /* [R, D] */
+    void* r_out;                  /* [R, D] with r */
+    float* rstd;                  /* [R]; forward: may be NULL */
+    float* scale;                 /* with fp8 */
+    const void* v;                /* [R, D]: r_out, or x without a residual stream (backward from here) */
+    const void* dy;               /* [R, D] type of x */
+    const void* dr_out;           /* [R, D] type of r, or NULL */
+    void* dx;                     /* [R, D] type of x */
+    void* dr;                     /* [R, D] type of r, or NULL where it is dx */
+    float* part_w;                /* workspace [cula_kda_add_rms_norm_shares(), D] */
+    float* dw;                    /* [D] */
+    long long R;
+    long long x_row, r_row;       /* elements from a row of x, r to the next */
+    int D, group;
+    int fp32, res;
+    int fp8;
+    float eps;
+} cula_kda_add_rms_norm_args;
+int cula_kda_add_rms_norm_fwd(const cula_kda_add_rms_norm_args* args, void* stream);
+int cula_kda_add_rms_norm_bwd(const cula_kda_add_rms_norm_args* args, void* stream);
+int cula_kda_add_rms_norm_shares(int D, long long R);
+
 /*
  * Self-test of the bounded waits: launches one warp that waits on a barrier nothing completes; after max_polls
  * polls (1 .. 2^22) the wait gives up, *d_status is set to 1 (the time-out status every kernel above reports through
