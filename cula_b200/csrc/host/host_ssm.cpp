@@ -1,4 +1,6 @@
 // The operators of a selective state space block (selective scan, single-token steps, residual RMS norm) on the native host path.
+#include <climits>
+
 #include "host_common.h"
 
 namespace cula_host {
@@ -43,7 +45,7 @@ bool rows_fit(const Tensor& t, int64_t inner_dims, int64_t align_elements, uintp
         expect *= t.size(d);
     }
     for (int64_t d = 0; d < t.dim() - inner_dims; ++d)
-        if (t.size(d) != 1 && t.stride(d) % align_elements) return false;
+        if (t.size(d) != 1 && (t.stride(d) % align_elements || t.stride(d) > INT_MAX && d > 0)) return false;       // from token to token: 32 bits
     return aligned(t, align_bytes);
 }
 Tensor rows_of(const Tensor& t, int64_t inner_dims) {

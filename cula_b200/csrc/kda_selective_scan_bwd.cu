@@ -18,9 +18,12 @@ struct SelBwdSmem {
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float2 dy[2][G::LC][G::CH / 2];
     float4 b[2][G::LC][SL], c[2][G::LC][SL];
-    float2 sums[2][G::LC][G::CH];                                    // per channel: sum_n g B, sum_n w A (log2 units)
+    float4 sums[2][G::LC][G::CH / 2];                                // two channels' sum_n g B, sum_n w A (log2 units)
     float bc[2][SEL_WARPS][G::LC][2 * G::SP];                        // per warp: dB, dC
-    uint4 raw[3][4][Q][G::ITEMS];                                 // x, dt, z, dout rows as they are
+    float par[2][G::CH];                                             // dt_bias, skip
+    T raw_b[2][G::UNITS][4], raw_c[2][G::UNITS][4];                  // B and C rows as they are
+    uint4 raw[2][4][Q][G::ITEMS];                                    // x, dt, z, dout rows as they are
+    float4 kept[2][G::LC / SEL_KEEP][2][SEL_THREADS];                // each thread's states before every eighth token
     float4 acc[4][SEL_THREADS];                                      // a thread's sums for dskip and dbias (8 channels each)
 };
 
@@ -39,7 +42,7 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
     pdl_launch_dependents();
     pdl_wait();
 
-    const int cl = lane & (CL - 1), s = lane / CL, n0 = 4 * s, pair = warp * CL + cl, dc = d0 + 2 * pair;
+    const int cl = lane & (CL - 1), s = lane / CL, n0 = 4 * s, pair = warp * CL + cl, dc = d0 + 8 * cl + 2 * warp;
     const bool own = dc < d_end;
     float2 A2[2][2], dA[2][2];
 #pragma unroll
@@ -57,6 +60,14 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
 #pragma unroll
         for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
+
+    for (int i = tid; i < CH; i += SEL_THREADS) {
+        sm.par[0][i] = a.dt_bias && d0 + i < d_end ? a.dt_bias[d0 + i] : 0.f;
+        sm.par[1][i] = a.skip && d0 + i < d_end ? a.skip[d0 + i] : 0.f;
+    }
+    __syncthreads();
+    auto param = [&](int which, float2 (&v)[4]) { SelVec<float>::unpack(reinterpret_cast<const uint4*>(&sm.par[which][dv - d0]), 1, v); };
+    const int x_row = (int)a.x_row, dt_row = (int)a.dt_row, z_row = (int)a.z_row, b_row = (int)a.b_row, c_row = (int)a.c_row;
 
     for (long long i = row; i < items; i += a.cta_rows) {
         SelItem it;
@@ -99,58 +110,76 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
         auto fetch = [&](int j) {
             const int t = it.t0 + (n_tiles - 1 - j) * LC + tt;
             if (item && j < n_tiles && t < it.t1) {
-                uint4(*to)[Q][G::ITEMS] = sm.raw[j % 3];
+                uint4(*to)[Q][G::ITEMS] = sm.raw[j & 1];
 #pragma unroll
                 for (int q = 0; q < Q; ++q) {
-                    sel_copy16(&to[0][q][tid], xp + (long long)t * a.x_row + q * (8 / Q));
-                    sel_copy16(&to[1][q][tid], dtp + (long long)t * a.dt_row + q * (8 / Q));
-                    if (gate) sel_copy16(&to[2][q][tid], zp + (long long)t * a.z_row + q * (8 / Q));
+                    sel_copy16(&to[0][q][tid], xp + (long long)t * x_row + q * (8 / Q));
+                    sel_copy16(&to[1][q][tid], dtp + (long long)t * dt_row + q * (8 / Q));
+                    if (gate) sel_copy16(&to[2][q][tid], zp + (long long)t * z_row + q * (8 / Q));
                     sel_copy16(&to[3][q][tid], dop + (size_t)t * a.D + q * (8 / Q));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < G::UB; ++u) {
+                const int i = u * SEL_THREADS + tid, t = it.t0 + (n_tiles - 1 - j) * LC + i / SL;
+                if (i < G::UNITS && j < n_tiles && t < it.t1) {
+                    if (!STATE_ONLY) sel_fetch4(sm.raw_b[j & 1][i], bp + (long long)t * b_row, 4 * (i % SL), a.S, a.vec_bc);
+                    sel_fetch4(sm.raw_c[j & 1][i], cp + (long long)t * c_row, 4 * (i % SL), a.S, a.vec_bc);
+                }
+            }
+            if (!STATE_ONLY && own && j < n_tiles) {
+#pragma unroll
+                for (int sub = 0; sub < LC / KEEP; ++sub) {
+                    const int at = it.t0 + (n_tiles - 1 - j) * LC + sub * KEEP;
+                    if (at < it.t1) {
+                        const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + at / KEEP) * a.D + dc) * SP + n0;
+                        sel_copy16(&sm.kept[j & 1][sub][0][tid], from);
+                        sel_copy16(&sm.kept[j & 1][sub][1][tid], from + SP);
+                    }
                 }
             }
             sel_commit();
         };
-        float4 rb[G::UB], rc[G::UB];
-        auto fetch_bc = [&](int j) {
-#pragma unroll
-            for (int u = 0; u < G::UB; ++u) {
-                const int i = u * SEL_THREADS + tid, t = it.t0 + (n_tiles - 1 - j) * LC + i / SL;
-                const bool ok = i < G::UNITS && j < n_tiles && t < it.t1;
-                if (!STATE_ONLY) rb[u] = ok ? sel_four(bp + (long long)t * a.b_row, 4 * (i % SL), a.S, a.vec_bc) : make_float4(0.f, 0.f, 0.f, 0.f);
-                rc[u] = ok ? sel_four(cp + (long long)t * a.c_row, 4 * (i % SL), a.S, a.vec_bc) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        };
         auto stage = [&](int j) {
-            const int buf = j & 1;
+            const int buf = j & 1, t_first = it.t0 + (n_tiles - 1 - j) * LC;
             if (tid < G::ITEMS) {                                    // zeros for channels past the tile: they add nothing to dB and dC
-                const bool live = item && it.t0 + (n_tiles - 1 - j) * LC + tt < it.t1;
-                float2 x[4], d[4], z[4], o[4];
-                if (live) {
-                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j % 3];
-                    V::unpack(&from[0][0][tid], G::ITEMS, x);
-                    V::unpack(&from[1][0][tid], G::ITEMS, d);
-                    if (gate) V::unpack(&from[2][0][tid], G::ITEMS, z);
-                    V::unpack(&from[3][0][tid], G::ITEMS, o);
+                const bool live = item && t_first + tt < it.t1;
+                const uint4(*from)[Q][G::ITEMS] = sm.raw[buf];
+                float2 x[4], d[4], o[4], b[4];
+                V::unpack(&from[0][0][tid], G::ITEMS, x);
+                V::unpack(&from[1][0][tid], G::ITEMS, d);
+                V::unpack(&from[3][0][tid], G::ITEMS, o);
+                param(0, b);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = add2(d[e], b[e]);
+                if (a.softplus) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[e] = sel_softplus2(d[e]);
+                }
+                if (gate) {
+                    float2 z[4];
+                    V::unpack(&from[2][0][tid], G::ITEMS, z);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = mul2(mul2(o[e], z[e]), sel_sigmoid2(z[e]));
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float2 step = make_float2(0.f, 0.f), prod = step, dy = step;
-                    if (live) {
-                        step = a.dt_bias ? add2(d[e], *reinterpret_cast<const float2*>(a.dt_bias + dv + 2 * e)) : d[e];
-                        if (a.softplus) step = softplus2(step);
-                        prod = mul2(step, x[e]);
-                        dy = gate ? mul2(mul2(o[e], z[e]), sel_sigmoid2(z[e])) : o[e];
-                    }
-                    sm.dx[buf][tt][vec * 4 + e] = make_float4(step.x, step.y, prod.x, prod.y);
-                    sm.dy[buf][tt][vec * 4 + e] = dy;
+                    const float2 p = mul2(d[e], x[e]);
+                    sm.dx[buf][tt][e * G::VECS + vec] = live ? make_float4(d[e].x, d[e].y, p.x, p.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    sm.dy[buf][tt][e * G::VECS + vec] = live ? o[e] : make_float2(0.f, 0.f);
                 }
             }
 #pragma unroll
             for (int u = 0; u < G::UB; ++u) {
                 const int i = u * SEL_THREADS + tid;
                 if (i < G::UNITS) {
-                    if (!STATE_ONLY) sm.b[buf][i / SL][i % SL] = rb[u];
-                    sm.c[buf][i / SL][i % SL] = rc[u];
+                    const bool live = t_first + i / SL < it.t1;
+                    if (!STATE_ONLY) {
+                        const float4 rb = V::four(sm.raw_b[buf][i]);
+                        sm.b[buf][i / SL][i % SL] = live ? rb : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    const float4 rc = V::four(sm.raw_c[buf][i]);
+                    sm.c[buf][i / SL][i % SL] = live ? rc : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
         };
@@ -159,15 +188,12 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
         if (n_tiles > 0) {
             fetch(0);
             fetch(1);
-            fetch_bc(0);
             sel_wait<1>();
             stage(0);
             __syncthreads();
         }
         for (int j = 0; j < n_tiles; ++j) {
             const int buf = j & 1, tile_t0 = it.t0 + (n_tiles - 1 - j) * LC;
-            fetch(j + 2);
-            fetch_bc(j + 1);
             if constexpr (STATE_ONLY) {
 #pragma unroll 8
                 for (int u = LC - 1; u >= 0; --u) {
@@ -187,14 +213,11 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                     const int tb = sub * KEEP;
                     if (tile_t0 + tb >= it.t1) continue;             // past the end: nothing in it
                     float2 st[KEEP + 1][2][2], av[KEEP][2][2];       // states before and after each token; a_t
-                    {
-                        const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + (tile_t0 + tb) / KEEP) * a.D + dc) * SP + n0;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const float4 r = own ? *reinterpret_cast<const float4*>(from + c * SP) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            st[0][c][0] = make_float2(r.x, r.y);
-                            st[0][c][1] = make_float2(r.z, r.w);
-                        }
+                    for (int c = 0; c < 2; ++c) {
+                        const float4 r = own ? sm.kept[buf][sub][c][tid] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        st[0][c][0] = make_float2(r.x, r.y);
+                        st[0][c][1] = make_float2(r.z, r.w);
                     }
 #pragma unroll
                     for (int u = 0; u < KEEP; ++u) {
@@ -213,10 +236,19 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                     for (int c = 0; c < 2; ++c) dA8[c][0] = dA8[c][1] = make_float2(0.f, 0.f);
                     constexpr int TB = SL > 4 ? SL / 4 : 1;          // tokens whose sums over states are added up together
                     float v[4 * TB];
+                    // the next token's rows are asked for before this one's sums are stored: no load waits behind a store
+                    float4 dx_n = sm.dx[buf][tb + KEEP - 1][pair], b_n = sm.b[buf][tb + KEEP - 1][s], c_n = sm.c[buf][tb + KEEP - 1][s];
+                    float2 dy_n = sm.dy[buf][tb + KEEP - 1][pair];
 #pragma unroll
                     for (int u = KEEP - 1; u >= 0; --u) {
-                        const float4 dx = sm.dx[buf][tb + u][pair], b = sm.b[buf][tb + u][s], cc = sm.c[buf][tb + u][s];
-                        const float2 dy = sm.dy[buf][tb + u][pair];
+                        const float4 dx = dx_n, b = b_n, cc = c_n;
+                        const float2 dy = dy_n;
+                        if (u > 0) {
+                            dx_n = sm.dx[buf][tb + u - 1][pair];
+                            b_n = sm.b[buf][tb + u - 1][s];
+                            c_n = sm.c[buf][tb + u - 1][s];
+                            dy_n = sm.dy[buf][tb + u - 1][pair];
+                        }
                         float2 dB0 = make_float2(0.f, 0.f), dB1 = dB0, dC0 = dB0, dC1 = dB0;
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -246,7 +278,7 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
 #pragma unroll
                             for (int k = 0; k < LEFT; ++k) {
                                 const int id = at + k, tok = id / 4, ch = (id >> 1) & 1, which = id & 1;
-                                reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][2 * pair + ch])[which] = r[k];
+                                reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][pair])[2 * ch + which] = r[k];
                             }
                         }
                         float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
@@ -274,41 +306,41 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                 }
             }
             if (j + 1 < n_tiles) {
-                sel_wait<1>();
+                sel_wait<0>();                                       // asked for one tile ago
                 stage(j + 1);
             }
             __syncthreads();
             if constexpr (!STATE_ONLY) {
                 const int t = tile_t0 + tt;
                 if (item && t < it.t1) {
-                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j % 3];
+                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j & 1];
                     const size_t at = (size_t)(it.row0 + t) * a.D + dv;
                     float2 x[4], d[4], o[4];
                     V::unpack(&from[0][0][tid], G::ITEMS, x);
                     V::unpack(&from[1][0][tid], G::ITEMS, d);
+                    float2 b[4], skip[4], sg[4];
+                    param(0, b);
+                    param(1, skip);
+                    if (a.softplus) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sg[e] = sel_sigmoid2(add2(d[e], b[e]));
+                    } else sg[0] = sg[1] = sg[2] = sg[3] = splat2(1.f);
                     float4 acc[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[e] = sm.acc[e][tid];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float4 step = sm.dx[buf][tt][vec * 4 + e];
-                        const float2 dy = sm.dy[buf][tt][vec * 4 + e];
-                        const float4 sums = *reinterpret_cast<const float4*>(&sm.sums[buf][tt][8 * vec + 2 * e]);
+                        const float4 step = sm.dx[buf][tt][e * G::VECS + vec], sums = sm.sums[buf][tt][e * G::VECS + vec];
+                        const float2 dy = sm.dy[buf][tt][e * G::VECS + vec];
                         const float2 gB = make_float2(sums.x, sums.z), wA = make_float2(sums.y, sums.w);
-                        float2 dd = fma2(x[e], gB, mul2(wA, splat2(0.6931471805599453f)));          // A is held times log2(e)
-                        if (a.softplus) {
-                            const float2 raw = a.dt_bias ? add2(d[e], *reinterpret_cast<const float2*>(a.dt_bias + dv + 2 * e)) : d[e];
-                            dd = mul2(dd, sel_sigmoid2(raw));
-                        }
-                        const float2 skip = a.skip ? *reinterpret_cast<const float2*>(a.skip + dv + 2 * e) : make_float2(0.f, 0.f);
-                        const float2 dxv = fma2(make_float2(step.x, step.y), gB, mul2(skip, dy));
+                        const float2 dd = mul2(fma2(x[e], gB, mul2(wA, splat2(0.6931471805599453f))), sg[e]);      // A is held times log2(e)
                         const float2 ds = mul2(dy, x[e]);
                         float4& as = acc[e / 2];
                         float4& ab = acc[2 + e / 2];
                         if (e & 1) { as.z += ds.x; as.w += ds.y; ab.z += dd.x; ab.w += dd.y; }
                         else { as.x += ds.x; as.y += ds.y; ab.x += dd.x; ab.y += dd.y; }
                         d[e] = dd;
-                        x[e] = dxv;
+                        x[e] = fma2(make_float2(step.x, step.y), gB, mul2(skip[e], dy));
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sm.acc[e][tid] = acc[e];
@@ -342,6 +374,7 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                     }
                 }
             }
+            fetch(j + 2);                                            // where tile j was
         }
         sel_wait<0>();
         __syncthreads();                                             // the next item stages into the same buffers

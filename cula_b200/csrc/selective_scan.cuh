@@ -6,7 +6,8 @@
 //
 // A thread holds two channels times four states; SL lanes share the states of a channel (SP = 4 SL of them, the ones past S are zero),
 // CL = 32 / SL lanes stand side by side over channels. The lanes of one state quad are neighbours, since a 16-byte shared load whose
-// neighbouring lanes ask for the same address takes 2.3 cycles of the SM instead of 4.
+// neighbouring lanes ask for the same address takes 2.3 cycles of the SM instead of 4. Lane cl of warp w has channels 8 cl + 2 w and the
+// next: what one thread stages, a piece of 8 channels, is a pair for each warp, and both sides touch shared memory in order.
 #pragma once
 #include "kda_common.cuh"
 #include "kda_params.h"
@@ -88,7 +89,6 @@ template <> struct SelVec<__nv_bfloat16> {
     __device__ static void store(__nv_bfloat16* p, const float2 (&v)[4]) {
         *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(v[0].x, v[0].y), pack_bf16(v[1].x, v[1].y), pack_bf16(v[2].x, v[2].y), pack_bf16(v[3].x, v[3].y));
     }
-    __device__ static float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
     __device__ static float4 four(const __nv_bfloat16* p) {
         const uint2 r = *reinterpret_cast<const uint2*>(p);
         const float2 a = unpack_bf16(r.x), b = unpack_bf16(r.y);
@@ -105,27 +105,29 @@ template <> struct SelVec<float> {
         reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
         reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     }
-    __device__ static float one(const float* p) { return *p; }
     __device__ static float4 four(const float* p) { return *reinterpret_cast<const float4*>(p); }
 };
 // Each thread copies the pieces that it will use itself, so their arrival concerns no other thread.
 __device__ __forceinline__ void sel_copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(smem_u32(dst)), "l"(src) : "memory");
 }
+template <int BYTES>
+__device__ __forceinline__ void sel_copy(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
 __device__ __forceinline__ void sel_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void sel_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
-// four states of a B or C row, zeros past the last of S
+// Four states of a B or C row, as they are, into the thread's own place: one copy where rows allow it, else element by element (zeros past
+// the last of S).
 template <typename T>
-__device__ __forceinline__ float4 sel_four(const T* row, int n, int S, int vec) {
-    if (vec && n + 3 < S) return SelVec<T>::four(row + n);
-    float4 r;
-    r.x = n < S ? SelVec<T>::one(row + n) : 0.f;
-    r.y = n + 1 < S ? SelVec<T>::one(row + n + 1) : 0.f;
-    r.z = n + 2 < S ? SelVec<T>::one(row + n + 2) : 0.f;
-    r.w = n + 3 < S ? SelVec<T>::one(row + n + 3) : 0.f;
-    return r;
+__device__ __forceinline__ void sel_fetch4(T* to, const T* row, int n, int S, int vec) {
+    if (vec && n + 3 < S) sel_copy<4 * sizeof(T)>(to, row + n);
+    else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to[k] = n + k < S ? row[n + k] : T(0.f);
+    }
 }
 // four states of a [.., S] fp32 row
 __device__ __forceinline__ void sel_load4(const float* row, int n, int S, float2 (&v)[2]) {
@@ -141,6 +143,21 @@ __device__ __forceinline__ void sel_store4(float* row, int n, int S, const float
         if (n + k < S) row[n + k] = f[k];
 }
 
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|), with log1p(e) = e q(e): q by Remez exchange for the least relative error on [0, 1]
+// (4.7e-9 before rounding, 1.7e-7 in fp32 arithmetic). One exponential and no reciprocal: the exponentials' unit bounds the scan.
+__device__ __forceinline__ float2 sel_softplus2(float2 x) {
+    const float2 e = ex2_2(make_float2(-RCP_LN2 * fabsf(x.x), -RCP_LN2 * fabsf(x.y)));
+    float2 q = fma2(e, splat2(-0.00324402517f), splat2(0.0198514629f));
+    q = fma2(e, q, splat2(-0.0569595359f));
+    q = fma2(e, q, splat2(0.106036551f));
+    q = fma2(e, q, splat2(-0.153055921f));
+    q = fma2(e, q, splat2(0.196759388f));
+    q = fma2(e, q, splat2(-0.249541342f));
+    q = fma2(e, q, splat2(0.333299637f));
+    q = fma2(e, q, splat2(-0.499999017f));
+    q = fma2(e, q, splat2(1.f));
+    return fma2(e, q, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
 __device__ __forceinline__ float2 sel_sigmoid2(float2 x) {
     return make_float2(fast_rcp(1.f + fast_exp2(-RCP_LN2 * x.x)), fast_rcp(1.f + fast_exp2(-RCP_LN2 * x.y)));
 }
