@@ -11,36 +11,254 @@
 
 namespace kda {
 
+constexpr int SEL_BWD_THREADS = 2 * SEL_THREADS;
+constexpr int SEL_SCAN_REGS = 184, SEL_SERVE_REGS = 72;             // of a thread of either kind; the block is launched with their mean
+
+__device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(SEL_BWD_THREADS) : "memory"); }
+
 template <int SL, typename T>
 struct SelBwdSmem {
     using G = SelShape<SL>;
-    static constexpr int Q = SelVec<T>::Q;
+    static constexpr int Q = SelVec<T>::Q, RING = Q == 1 ? 3 : 2;    // tiles of rows: of the gradients that are made, of the next tile, one more of 16 bits
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float2 dy[2][G::LC][G::CH / 2];
     float4 b[2][G::LC][SL], c[2][G::LC][SL];
     float4 sums[2][G::LC][G::CH / 2];                                // two channels' sum_n g B, sum_n w A (log2 units)
     float bc[2][SEL_WARPS][G::LC][2 * G::SP];                        // per warp: dB, dC
     float par[2][G::CH];                                             // dt_bias, skip
-    T raw_b[2][G::UNITS][4], raw_c[2][G::UNITS][4];                  // B and C rows as they are
-    uint4 raw[2][4][Q][G::ITEMS];                                    // x, dt, z, dout rows as they are
-    float4 kept[2][G::LC / SEL_KEEP][2][SEL_THREADS];                // each thread's states before every eighth token
-    float4 acc[4][SEL_THREADS];                                      // a thread's sums for dskip and dbias (8 channels each)
+    T raw_b[RING][G::UNITS][4], raw_c[RING][G::UNITS][4];            // B and C rows as they are
+    uint4 raw[RING][4][Q][G::ITEMS];                                 // x, dt, z, dout rows as they are
+    float4 kept[G::LC / SEL_KEEP][2][SEL_THREADS];                   // each thread's states before every eighth token
+    float4 acc[4][G::ITEMS];                                         // a thread's sums for dskip and dbias (8 channels each)
 };
+
+// What the serving warps do for an item: rows of the tiles to come, operands of the next tile, gradients of the one before.
+template <int SL, typename T, bool STATE_ONLY>
+__device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<SL, T>& sm, const SelItem& it, int d0, int d_end, int group, int share) {
+    using G = SelShape<SL>;
+    using V = SelVec<T>;
+    constexpr int LC = G::LC, SP = G::SP, Q = V::Q, RING = SelBwdSmem<SL, T>::RING;
+    const int tid = threadIdx.x % SEL_THREADS, tt = tid / G::VECS, vec = tid % G::VECS, dv = d0 + 8 * vec;
+    const bool item = tid < G::ITEMS && dv < d_end, gate = a.z != nullptr;
+    const int batch = a.cu_seqlens ? 0 : it.seq, n_tiles = (it.t1 - it.t0 + LC - 1) / LC;
+    const long long first = a.cu_seqlens ? it.row0 : 0;
+    const T* xp = static_cast<const T*>(a.x) + batch * a.x_seq + first * a.x_row + dv;
+    const T* dtp = static_cast<const T*>(a.dt) + batch * a.dt_seq + first * a.dt_row + dv;
+    const T* zp = static_cast<const T*>(a.z) + batch * a.z_seq + first * a.z_row + dv;
+    const T* dop = static_cast<const T*>(a.dy) + (size_t)it.row0 * a.D + dv;
+    const T* bp = static_cast<const T*>(a.Bm) + batch * a.b_seq + first * a.b_row + group * a.S;
+    const T* cp = static_cast<const T*>(a.Cm) + batch * a.c_seq + first * a.c_row + group * a.S;
+    const int x_row = (int)a.x_row, dt_row = (int)a.dt_row, z_row = (int)a.z_row, b_row = (int)a.b_row, c_row = (int)a.c_row;
+    auto param = [&](int which, float2 (&v)[4]) { SelVec<float>::unpack(reinterpret_cast<const uint4*>(&sm.par[which][8 * vec]), 1, v); };
+    // tiles are taken from the last to the first; the j-th taken is tile n_tiles - 1 - j
+    auto fetch = [&](int j) {
+        const int t_first = it.t0 + (n_tiles - 1 - j) * LC, t = t_first + tt, slot = j % RING;
+        if (item && j < n_tiles && t < it.t1) {
+            uint4(*to)[Q][G::ITEMS] = sm.raw[slot];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                sel_copy16(&to[0][q][tid], xp + (long long)t * x_row + q * (8 / Q));
+                sel_copy16(&to[1][q][tid], dtp + (long long)t * dt_row + q * (8 / Q));
+                if (gate) sel_copy16(&to[2][q][tid], zp + (long long)t * z_row + q * (8 / Q));
+                sel_copy16(&to[3][q][tid], dop + (size_t)t * a.D + q * (8 / Q));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < G::UB; ++u) {
+            const int i = u * SEL_THREADS + tid, tb = t_first + i / SL;
+            if (i < G::UNITS && j < n_tiles && tb < it.t1) {
+                if (!STATE_ONLY) sel_fetch4(sm.raw_b[slot][i], bp + (long long)tb * b_row, 4 * (i % SL), a.S, a.vec_bc);
+                sel_fetch4(sm.raw_c[slot][i], cp + (long long)tb * c_row, 4 * (i % SL), a.S, a.vec_bc);
+            }
+        }
+        sel_commit();
+    };
+    auto stage = [&](int j) {
+        const int buf = j & 1, t_first = it.t0 + (n_tiles - 1 - j) * LC, slot = j % RING;
+        if (tid < G::ITEMS) {                                        // zeros for channels past the tile: they add nothing to dB and dC
+            const bool live = item && t_first + tt < it.t1;
+            const uint4(*from)[Q][G::ITEMS] = sm.raw[slot];
+            float2 x[4], d[4], b[4];
+            V::unpack(&from[1][0][tid], G::ITEMS, d);
+            param(0, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = add2(d[e], b[e]);
+            if (a.softplus) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = sel_softplus2(d[e]);
+            }
+            V::unpack(&from[0][0][tid], G::ITEMS, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 p = mul2(d[e], x[e]);
+                sm.dx[buf][tt][e * G::VECS + vec] = live ? make_float4(d[e].x, d[e].y, p.x, p.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float2 o[4];
+            V::unpack(&from[3][0][tid], G::ITEMS, o);
+            if (gate) {
+                float2 z[4];
+                V::unpack(&from[2][0][tid], G::ITEMS, z);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = mul2(mul2(o[e], z[e]), sel_sigmoid2(z[e]));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sm.dy[buf][tt][e * G::VECS + vec] = live ? o[e] : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < G::UB; ++u) {
+            const int i = u * SEL_THREADS + tid;
+            if (i < G::UNITS) {
+                const bool live = t_first + i / SL < it.t1;
+                if (!STATE_ONLY) {
+                    const float4 rb = V::four(sm.raw_b[slot][i]);
+                    sm.b[buf][i / SL][i % SL] = live ? rb : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                const float4 rc = V::four(sm.raw_c[slot][i]);
+                sm.c[buf][i / SL][i % SL] = live ? rc : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+    };
+    auto finish = [&](int j) {
+        const int buf = j & 1, t_first = it.t0 + (n_tiles - 1 - j) * LC, t = t_first + tt;
+        if (item && t < it.t1) {
+            const uint4(*from)[Q][G::ITEMS] = sm.raw[j % RING];
+            const size_t at = (size_t)(it.row0 + t) * a.D + dv;
+            float4 y0, y1;
+            if (gate) {                                              // on its way while dx and ddt are made
+                y0 = reinterpret_cast<const float4*>(a.y_pre + at)[0];
+                y1 = reinterpret_cast<const float4*>(a.y_pre + at)[1];
+            }
+            float2 x[4], d[4], sg[4];
+            V::unpack(&from[1][0][tid], G::ITEMS, d);
+            if (a.softplus) {
+                float2 b[4];
+                param(0, b);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sg[e] = sel_sigmoid2(add2(d[e], b[e]));
+            } else sg[0] = sg[1] = sg[2] = sg[3] = splat2(1.f);
+            V::unpack(&from[0][0][tid], G::ITEMS, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 sums = sm.sums[buf][tt][e * G::VECS + vec];
+                d[e] = mul2(fma2(x[e], make_float2(sums.x, sums.z), mul2(make_float2(sums.y, sums.w), splat2(0.6931471805599453f))), sg[e]);      // A is held times log2(e)
+            }
+            V::store(static_cast<T*>(a.ddt) + at, d);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 ab = sm.acc[2 + h][tid];
+                ab.x += d[2 * h].x; ab.y += d[2 * h].y; ab.z += d[2 * h + 1].x; ab.w += d[2 * h + 1].y;
+                sm.acc[2 + h][tid] = ab;
+            }
+            param(1, d);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 as = sm.acc[h][tid];
+#pragma unroll
+                for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                    const float4 step = sm.dx[buf][tt][e * G::VECS + vec], sums = sm.sums[buf][tt][e * G::VECS + vec];
+                    const float2 dy = sm.dy[buf][tt][e * G::VECS + vec], ds = mul2(dy, x[e]);
+                    if (e & 1) { as.z += ds.x; as.w += ds.y; }
+                    else { as.x += ds.x; as.y += ds.y; }
+                    x[e] = fma2(make_float2(step.x, step.y), make_float2(sums.x, sums.z), mul2(d[e], dy));
+                }
+                sm.acc[h][tid] = as;
+            }
+            V::store(static_cast<T*>(a.dx) + at, x);
+            if (gate) {
+                float2 z[4], o[4];
+                V::unpack(&from[2][0][tid], G::ITEMS, z);
+                V::unpack(&from[3][0][tid], G::ITEMS, o);
+                const float2 y[4] = {make_float2(y0.x, y0.y), make_float2(y0.z, y0.w), make_float2(y1.x, y1.y), make_float2(y1.z, y1.w)};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 s = sel_sigmoid2(z[e]);             // silu' = s (1 + z (1 - s))
+                    o[e] = mul2(mul2(o[e], y[e]), mul2(s, fma2(z[e], fma2(s, splat2(-1.f), splat2(1.f)), splat2(1.f))));
+                }
+                V::store(static_cast<T*>(a.dz) + at, o);
+            }
+        }
+        // this tile of channels' share of dB and dC
+        for (int i = tid; i < LC * SP / 2; i += SEL_THREADS) {
+            const int u = i / (SP / 2), n = 4 * (i % (SP / 2));
+            if (t_first + u < it.t1) {
+                float4 sum = *reinterpret_cast<const float4*>(&sm.bc[buf][0][u][n]);
+#pragma unroll
+                for (int w = 1; w < SEL_WARPS; ++w) {
+                    const float4 r = *reinterpret_cast<const float4*>(&sm.bc[buf][w][u][n]);
+                    sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
+                }
+                const size_t at = (((size_t)share * a.rows + it.row0 + t_first + u) * a.G + group) * (2 * SP) + n;
+                *reinterpret_cast<float4*>(a.part_bc + at) = sum;
+            }
+        }
+    };
+    if (n_tiles == 0) return;
+#pragma unroll
+    for (int j = 0; j < RING - 1; ++j) fetch(j);
+    sel_wait<RING - 2>();
+    stage(0);
+    sel_bwd_barrier();
+    for (int j = 0; j < n_tiles; ++j) {
+        if (!STATE_ONLY && j > 0) finish(j - 1);
+        fetch(j + RING - 1);                                         // where tile j - 1 was
+        sel_wait<RING - 2>();                                        // tile j + 1 is here
+        if (j + 1 < n_tiles) stage(j + 1);
+        sel_bwd_barrier();
+    }
+    if (!STATE_ONLY) finish(n_tiles - 1);
+    sel_wait<0>();
+}
 
 // STATE_ONLY: what each segment adds to the gradient of the state that leaves it, and the sum of its steps
 template <int SL, typename T, bool STATE_ONLY>
-__global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective_scan_bwd_kernel(const SelScanArgs a, const int tiles_per_group, const long long items) {
+__global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_kernel(const SelScanArgs a, const int tiles_per_group, const long long items) {
     using G = SelShape<SL>;
-    using V = SelVec<T>;
-    constexpr int LC = G::LC, CH = G::CH, CL = G::CL, SP = G::SP, Q = V::Q, KEEP = SEL_KEEP;
+    constexpr int LC = G::LC, CH = G::CH, CL = G::CL, SP = G::SP, KEEP = SEL_KEEP, SUBS = LC / KEEP;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SelBwdSmem<SL, T>& sm = *reinterpret_cast<SelBwdSmem<SL, T>*>(smem_raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x % SEL_THREADS, lane = tid & 31, warp = tid >> 5;
     const int tiles = tiles_per_group * a.G, tile = blockIdx.x % tiles, row = blockIdx.x / tiles;
-    const int group = tile / tiles_per_group, per_group = a.D / a.G;
-    const int d0 = group * per_group + (tile % tiles_per_group) * CH, d_end = (group + 1) * per_group;
+    const int group = tile / tiles_per_group, per_group = a.D / a.G, share = tile % tiles_per_group;
+    const int d0 = group * per_group + share * CH, d_end = (group + 1) * per_group;
     pdl_launch_dependents();
     pdl_wait();
+
+    if (threadIdx.x >= SEL_THREADS) {
+        // Of the 128 registers per thread that the block starts with, the serving warps give up what the scanning ones need
+        if constexpr (!STATE_ONLY) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(SEL_SERVE_REGS));
+        for (int i = tid; i < CH; i += SEL_THREADS) {
+            sm.par[0][i] = a.dt_bias && d0 + i < d_end ? a.dt_bias[d0 + i] : 0.f;
+            sm.par[1][i] = a.skip && d0 + i < d_end ? a.skip[d0 + i] : 0.f;
+        }
+        if (!STATE_ONLY && tid < G::ITEMS) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
+        for (long long i = row; i < items; i += a.cta_rows) {
+            SelItem it;
+            if (!sel_item(a, i, it) || (STATE_ONLY && it.seg == 0)) continue;
+            sel_bwd_serve<SL, T, STATE_ONLY>(a, sm, it, d0, d_end, group, share);
+        }
+        if constexpr (!STATE_ONLY) {
+            asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
+            // dskip and dbias: the threads that stood at the same channels, in order
+            for (int i = tid; i < 4 * G::VECS; i += SEL_THREADS) {
+                const int v = i % G::VECS, e = i / G::VECS;
+                if (d0 + 8 * v < d_end) {
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = v; k < G::ITEMS; k += G::VECS) {
+                        const float4 r = sm.acc[e][k];
+                        sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
+                    }
+                    float* to = e < 2 ? a.part_skip : a.part_bias;
+                    if (to) *reinterpret_cast<float4*>(to + (size_t)row * a.D + d0 + 8 * v + 4 * (e & 1)) = sum;
+                }
+            }
+        }
+        return;
+    }
+    if constexpr (!STATE_ONLY) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(SEL_SCAN_REGS));
 
     const int cl = lane & (CL - 1), s = lane / CL, n0 = 4 * s, pair = warp * CL + cl, dc = d0 + 8 * cl + 2 * warp;
     const bool own = dc < d_end;
@@ -54,34 +272,25 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
             A2[c][1] = mul2(A2[c][1], splat2(RCP_LN2));
         }
     }
-    const int tt = tid / G::VECS, vec = tid % G::VECS, dv = d0 + 8 * vec;
-    const bool item = tid < G::ITEMS && dv < d_end, gate = a.z != nullptr;
-    if constexpr (!STATE_ONLY) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-
-    for (int i = tid; i < CH; i += SEL_THREADS) {
-        sm.par[0][i] = a.dt_bias && d0 + i < d_end ? a.dt_bias[d0 + i] : 0.f;
-        sm.par[1][i] = a.skip && d0 + i < d_end ? a.skip[d0 + i] : 0.f;
-    }
-    __syncthreads();
-    auto param = [&](int which, float2 (&v)[4]) { SelVec<float>::unpack(reinterpret_cast<const uint4*>(&sm.par[which][dv - d0]), 1, v); };
-    const int x_row = (int)a.x_row, dt_row = (int)a.dt_row, z_row = (int)a.z_row, b_row = (int)a.b_row, c_row = (int)a.c_row;
 
     for (long long i = row; i < items; i += a.cta_rows) {
         SelItem it;
-        if (!sel_item(a, i, it)) continue;
-        if (STATE_ONLY && it.seg == 0) continue;                     // nothing comes before it
-        const int batch = a.cu_seqlens ? 0 : it.seq;
-        const long long first = a.cu_seqlens ? it.row0 : 0;
-        const T* xp = static_cast<const T*>(a.x) + batch * a.x_seq + first * a.x_row + dv;
-        const T* dtp = static_cast<const T*>(a.dt) + batch * a.dt_seq + first * a.dt_row + dv;
-        const T* zp = static_cast<const T*>(a.z) + batch * a.z_seq + first * a.z_row + dv;
-        const T* dop = static_cast<const T*>(a.dy) + (size_t)it.row0 * a.D + dv;
-        const T* bp = static_cast<const T*>(a.Bm) + batch * a.b_seq + first * a.b_row + group * a.S;
-        const T* cp = static_cast<const T*>(a.Cm) + batch * a.c_seq + first * a.c_row + group * a.S;
+        if (!sel_item(a, i, it) || (STATE_ONLY && it.seg == 0)) continue;        // nothing comes before a first segment
         const int n_tiles = (it.t1 - it.t0 + LC - 1) / LC;
+        // the kept states of place `sub` of the j-th tile taken
+        auto fetch = [&](int j, int sub) {
+            const int at = it.t0 + (n_tiles - 1 - j) * LC + sub * KEEP;
+            if (own && j < n_tiles && at < it.t1) {
+                const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + at / KEEP) * a.D + dc) * SP + n0;
+                sel_copy16(&sm.kept[sub][0][tid], from);
+                sel_copy16(&sm.kept[sub][1][tid], from + SP);
+            }
+            sel_commit();
+        };
+        if constexpr (!STATE_ONLY) {
+#pragma unroll
+            for (int sub = SUBS - 1; sub >= 0; --sub) fetch(0, sub);
+        }
 
         float2 gh[2][2];                                             // a_{t+1} g_{t+1}: the gradient of h_t through what comes after
 #pragma unroll
@@ -106,96 +315,12 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
             }
         }
 
-        // tiles are taken from the last to the first; the j-th taken is tile n_tiles - 1 - j
-        auto fetch = [&](int j) {
-            const int t = it.t0 + (n_tiles - 1 - j) * LC + tt;
-            if (item && j < n_tiles && t < it.t1) {
-                uint4(*to)[Q][G::ITEMS] = sm.raw[j & 1];
-#pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    sel_copy16(&to[0][q][tid], xp + (long long)t * x_row + q * (8 / Q));
-                    sel_copy16(&to[1][q][tid], dtp + (long long)t * dt_row + q * (8 / Q));
-                    if (gate) sel_copy16(&to[2][q][tid], zp + (long long)t * z_row + q * (8 / Q));
-                    sel_copy16(&to[3][q][tid], dop + (size_t)t * a.D + q * (8 / Q));
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < G::UB; ++u) {
-                const int i = u * SEL_THREADS + tid, t = it.t0 + (n_tiles - 1 - j) * LC + i / SL;
-                if (i < G::UNITS && j < n_tiles && t < it.t1) {
-                    if (!STATE_ONLY) sel_fetch4(sm.raw_b[j & 1][i], bp + (long long)t * b_row, 4 * (i % SL), a.S, a.vec_bc);
-                    sel_fetch4(sm.raw_c[j & 1][i], cp + (long long)t * c_row, 4 * (i % SL), a.S, a.vec_bc);
-                }
-            }
-            if (!STATE_ONLY && own && j < n_tiles) {
-#pragma unroll
-                for (int sub = 0; sub < LC / KEEP; ++sub) {
-                    const int at = it.t0 + (n_tiles - 1 - j) * LC + sub * KEEP;
-                    if (at < it.t1) {
-                        const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + at / KEEP) * a.D + dc) * SP + n0;
-                        sel_copy16(&sm.kept[j & 1][sub][0][tid], from);
-                        sel_copy16(&sm.kept[j & 1][sub][1][tid], from + SP);
-                    }
-                }
-            }
-            sel_commit();
-        };
-        auto stage = [&](int j) {
-            const int buf = j & 1, t_first = it.t0 + (n_tiles - 1 - j) * LC;
-            if (tid < G::ITEMS) {                                    // zeros for channels past the tile: they add nothing to dB and dC
-                const bool live = item && t_first + tt < it.t1;
-                const uint4(*from)[Q][G::ITEMS] = sm.raw[buf];
-                float2 x[4], d[4], o[4], b[4];
-                V::unpack(&from[0][0][tid], G::ITEMS, x);
-                V::unpack(&from[1][0][tid], G::ITEMS, d);
-                V::unpack(&from[3][0][tid], G::ITEMS, o);
-                param(0, b);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) d[e] = add2(d[e], b[e]);
-                if (a.softplus) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[e] = sel_softplus2(d[e]);
-                }
-                if (gate) {
-                    float2 z[4];
-                    V::unpack(&from[2][0][tid], G::ITEMS, z);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = mul2(mul2(o[e], z[e]), sel_sigmoid2(z[e]));
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 p = mul2(d[e], x[e]);
-                    sm.dx[buf][tt][e * G::VECS + vec] = live ? make_float4(d[e].x, d[e].y, p.x, p.y) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    sm.dy[buf][tt][e * G::VECS + vec] = live ? o[e] : make_float2(0.f, 0.f);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < G::UB; ++u) {
-                const int i = u * SEL_THREADS + tid;
-                if (i < G::UNITS) {
-                    const bool live = t_first + i / SL < it.t1;
-                    if (!STATE_ONLY) {
-                        const float4 rb = V::four(sm.raw_b[buf][i]);
-                        sm.b[buf][i / SL][i % SL] = live ? rb : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                    const float4 rc = V::four(sm.raw_c[buf][i]);
-                    sm.c[buf][i / SL][i % SL] = live ? rc : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-            }
-        };
-
         float2 sum_dt = make_float2(0.f, 0.f);
-        if (n_tiles > 0) {
-            fetch(0);
-            fetch(1);
-            sel_wait<1>();
-            stage(0);
-            __syncthreads();
-        }
+        if (n_tiles > 0) sel_bwd_barrier();
         for (int j = 0; j < n_tiles; ++j) {
             const int buf = j & 1, tile_t0 = it.t0 + (n_tiles - 1 - j) * LC;
             if constexpr (STATE_ONLY) {
-#pragma unroll 8
+#pragma unroll
                 for (int u = LC - 1; u >= 0; --u) {
                     const float4 dx = sm.dx[buf][u][pair], cc = sm.c[buf][u][s];
                     const float2 dy = sm.dy[buf][u][pair];
@@ -209,16 +334,18 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                 }
             } else {
 #pragma unroll 1
-                for (int sub = LC / KEEP - 1; sub >= 0; --sub) {
+                for (int sub = SUBS - 1; sub >= 0; --sub) {
                     const int tb = sub * KEEP;
-                    if (tile_t0 + tb >= it.t1) continue;             // past the end: nothing in it
                     float2 st[KEEP + 1][2][2], av[KEEP][2][2];       // states before and after each token; a_t
+                    sel_wait<SUBS - 1>();
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float4 r = own ? sm.kept[buf][sub][c][tid] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float4 r = own ? sm.kept[sub][c][tid] : make_float4(0.f, 0.f, 0.f, 0.f);
                         st[0][c][0] = make_float2(r.x, r.y);
                         st[0][c][1] = make_float2(r.z, r.w);
                     }
+                    fetch(j + 1, sub);
+                    if (tile_t0 + tb >= it.t1) continue;             // past the end: nothing in it
 #pragma unroll
                     for (int u = 0; u < KEEP; ++u) {
                         const float4 dx = sm.dx[buf][tb + u][pair], b = sm.b[buf][tb + u][s];
@@ -231,9 +358,6 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                             st[u + 1][c][1] = fma2(p, make_float2(b.z, b.w), mul2(av[u][c][1], st[u][c][1]));
                         }
                     }
-                    float2 dA8[2][2];                                // eight terms are added up first
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) dA8[c][0] = dA8[c][1] = make_float2(0.f, 0.f);
                     constexpr int TB = SL > 4 ? SL / 4 : 1;          // tokens whose sums over states are added up together
                     float v[4 * TB];
                     // the next token's rows are asked for before this one's sums are stored: no load waits behind a store
@@ -254,17 +378,17 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                         for (int c = 0; c < 2; ++c) {
                             const float2 d = splat2(c ? dx.y : dx.x), p = splat2(c ? dx.w : dx.z), o = splat2(c ? dy.y : dy.x);
                             const float2 g0 = fma2(o, make_float2(cc.x, cc.y), gh[c][0]), g1 = fma2(o, make_float2(cc.z, cc.w), gh[c][1]);
-                            dC0 = fma2(o, st[u + 1][c][0], dC0);
-                            dC1 = fma2(o, st[u + 1][c][1], dC1);
-                            dB0 = fma2(g0, p, dB0);
-                            dB1 = fma2(g1, p, dB1);
+                            dC0 = c ? fma2(o, st[u + 1][c][0], dC0) : mul2(o, st[u + 1][c][0]);
+                            dC1 = c ? fma2(o, st[u + 1][c][1], dC1) : mul2(o, st[u + 1][c][1]);
+                            dB0 = c ? fma2(g0, p, dB0) : mul2(g0, p);
+                            dB1 = c ? fma2(g1, p, dB1) : mul2(g1, p);
                             const float2 s1 = fma2(g1, make_float2(b.z, b.w), mul2(g0, make_float2(b.x, b.y)));
                             gh[c][0] = mul2(av[u][c][0], g0);
                             gh[c][1] = mul2(av[u][c][1], g1);
                             const float2 w0 = mul2(gh[c][0], st[u][c][0]), w1 = mul2(gh[c][1], st[u][c][1]);
                             const float2 s2 = fma2(w1, A2[c][1], mul2(w0, A2[c][0]));
-                            dA8[c][0] = fma2(w0, d, dA8[c][0]);
-                            dA8[c][1] = fma2(w1, d, dA8[c][1]);
+                            dA[c][0] = fma2(w0, d, dA[c][0]);
+                            dA[c][1] = fma2(w1, d, dA[c][1]);
                             v[4 * (u % TB) + 2 * c] = s1.x + s1.y;
                             v[4 * (u % TB) + 2 * c + 1] = s2.x + s2.y;
                         }
@@ -298,86 +422,11 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
                             }
                         }
                     }
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        dA[c][0] = add2(dA[c][0], dA8[c][0]);
-                        dA[c][1] = add2(dA[c][1], dA8[c][1]);
-                    }
                 }
             }
-            if (j + 1 < n_tiles) {
-                sel_wait<0>();                                       // asked for one tile ago
-                stage(j + 1);
-            }
-            __syncthreads();
-            if constexpr (!STATE_ONLY) {
-                const int t = tile_t0 + tt;
-                if (item && t < it.t1) {
-                    const uint4(*from)[Q][G::ITEMS] = sm.raw[j & 1];
-                    const size_t at = (size_t)(it.row0 + t) * a.D + dv;
-                    float2 x[4], d[4], o[4];
-                    V::unpack(&from[0][0][tid], G::ITEMS, x);
-                    V::unpack(&from[1][0][tid], G::ITEMS, d);
-                    float2 b[4], skip[4], sg[4];
-                    param(0, b);
-                    param(1, skip);
-                    if (a.softplus) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sg[e] = sel_sigmoid2(add2(d[e], b[e]));
-                    } else sg[0] = sg[1] = sg[2] = sg[3] = splat2(1.f);
-                    float4 acc[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[e] = sm.acc[e][tid];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float4 step = sm.dx[buf][tt][e * G::VECS + vec], sums = sm.sums[buf][tt][e * G::VECS + vec];
-                        const float2 dy = sm.dy[buf][tt][e * G::VECS + vec];
-                        const float2 gB = make_float2(sums.x, sums.z), wA = make_float2(sums.y, sums.w);
-                        const float2 dd = mul2(fma2(x[e], gB, mul2(wA, splat2(0.6931471805599453f))), sg[e]);      // A is held times log2(e)
-                        const float2 ds = mul2(dy, x[e]);
-                        float4& as = acc[e / 2];
-                        float4& ab = acc[2 + e / 2];
-                        if (e & 1) { as.z += ds.x; as.w += ds.y; ab.z += dd.x; ab.w += dd.y; }
-                        else { as.x += ds.x; as.y += ds.y; ab.x += dd.x; ab.y += dd.y; }
-                        d[e] = dd;
-                        x[e] = fma2(make_float2(step.x, step.y), gB, mul2(skip[e], dy));
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sm.acc[e][tid] = acc[e];
-                    V::store(static_cast<T*>(a.dx) + at, x);
-                    V::store(static_cast<T*>(a.ddt) + at, d);
-                    if (gate) {
-                        float2 z[4];
-                        V::unpack(&from[2][0][tid], G::ITEMS, z);
-                        V::unpack(&from[3][0][tid], G::ITEMS, o);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 y = *reinterpret_cast<const float2*>(a.y_pre + at + 2 * e), sg = sel_sigmoid2(z[e]);
-                            // silu' = s (1 + z (1 - s))
-                            o[e] = mul2(mul2(o[e], y), mul2(sg, fma2(z[e], fma2(sg, splat2(-1.f), splat2(1.f)), splat2(1.f))));
-                        }
-                        V::store(static_cast<T*>(a.dz) + at, o);
-                    }
-                }
-                // this tile of channels' share of dB and dC
-                for (int i = tid; i < LC * SP / 2; i += SEL_THREADS) {
-                    const int u = i / (SP / 2), n = 4 * (i % (SP / 2));
-                    if (tile_t0 + u < it.t1) {
-                        float4 sum = *reinterpret_cast<const float4*>(&sm.bc[buf][0][u][n]);
-#pragma unroll
-                        for (int w = 1; w < SEL_WARPS; ++w) {
-                            const float4 r = *reinterpret_cast<const float4*>(&sm.bc[buf][w][u][n]);
-                            sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
-                        }
-                        const size_t at = (((size_t)(tile % tiles_per_group) * a.rows + it.row0 + tile_t0 + u) * a.G + group) * (2 * SP) + n;
-                        *reinterpret_cast<float4*>(a.part_bc + at) = sum;
-                    }
-                }
-            }
-            fetch(j + 2);                                            // where tile j was
+            sel_bwd_barrier();
         }
         sel_wait<0>();
-        __syncthreads();                                             // the next item stages into the same buffers
         if (own) {
             if constexpr (STATE_ONLY) {
                 const size_t at = (size_t)(it.slot0 + it.seg) * a.D + dc;
@@ -396,20 +445,6 @@ __global__ void __launch_bounds__(SEL_THREADS, STATE_ONLY ? 4 : 2) kda_selective
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 *reinterpret_cast<float4*>(a.part_A + ((size_t)row * a.D + dc + c) * SP + n0) = make_float4(dA[c][0].x, dA[c][0].y, dA[c][1].x, dA[c][1].y);
-        }
-        __syncthreads();
-        // dskip and dbias: the threads that stood at the same channels, in order
-        for (int i = tid; i < 4 * G::VECS; i += SEL_THREADS) {
-            const int v = i % G::VECS, e = i / G::VECS;
-            if (d0 + 8 * v < d_end) {
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = v; k < G::ITEMS; k += G::VECS) {
-                    const float4 r = sm.acc[e][k];
-                    sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
-                }
-                float* to = e < 2 ? a.part_skip : a.part_bias;
-                if (to) *reinterpret_cast<float4*>(to + (size_t)row * a.D + d0 + 8 * v + 4 * (e & 1)) = sum;
-            }
         }
     }
 }
@@ -469,12 +504,18 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> done[2];
     if (a.seg_chunks) {
         if (const cudaError_t e = allow_smem(kda_selective_scan_bwd_kernel<SL, T, true>, smem, done[1]); e != cudaSuccess) return (int)launched(e);
-        if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, true>, dim3((unsigned)blocks), SEL_THREADS, smem, stream, a, tpg, items);
+        if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, true>, dim3((unsigned)blocks), SEL_BWD_THREADS, smem, stream, a, tpg, items);
             e != cudaSuccess)
             return (int)e;
     }
     if (const cudaError_t e = allow_smem(kda_selective_scan_bwd_kernel<SL, T, false>, smem, done[0]); e != cudaSuccess) return (int)launched(e);
-    if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_THREADS, smem, stream, a, tpg, items);
+    // the scanning warps would wait for ever for registers that the block was not launched with
+    static const bool enough = [] {
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, kda_selective_scan_bwd_kernel<SL, T, false>) == cudaSuccess && 2 * f.numRegs >= SEL_SCAN_REGS + SEL_SERVE_REGS;
+    }();
+    if (!enough) return (int)cudaErrorLaunchOutOfResources;
+    if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_BWD_THREADS, smem, stream, a, tpg, items);
         e != cudaSuccess)
         return (int)e;
     const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 255) / 256, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
