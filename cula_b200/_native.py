@@ -59,6 +59,7 @@ SIGNATURES = {
     "cula_kda_selective_scan_fwd": (_i, [_vp, _vp]),
     "cula_kda_selective_scan_bwd": (_i, [_vp, _vp]),
     "cula_kda_selective_scan_tiles": (_i, [_i, _i, _i]),
+    "cula_kda_selective_scan_state_floats": (_i, [_i, _i, _i]),
     "cula_kda_selective_step": (_i, [_vp, _vp]),
     "cula_kda_conv_step": (_i, [_vp, _vp]),
     "cula_kda_add_rms_norm_fwd": (_i, [_vp, _vp]),

@@ -507,6 +507,11 @@ extern "C" int cula_kda_selective_scan_tiles(int D, int G, int S) {
     return D <= 0 || G <= 0 || S <= 0 || S > 64 ? CULA_KDA_EINVAL : kda_selective_scan_tiles(D, G, state_lanes(S));
 }
 
+extern "C" int cula_kda_selective_scan_state_floats(int D, int G, int S) {
+    const int tiles = cula_kda_selective_scan_tiles(D, G, S);
+    return tiles < 0 ? tiles : tiles * G * 1024;                     // 128 threads of a tile hold 8 each
+}
+
 extern "C" int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* a, void* stream) {
     if (const int e = scan_args_error(a)) return e;
     if (a->n_seqs == 0) return 0;

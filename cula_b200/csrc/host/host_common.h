@@ -30,7 +30,7 @@ enum { GATE_NONE = 0, GATE_SOFTPLUS = 1, GATE_LOWER_BOUND = 2 };
     X(cula_kda_bwd_dense) X(cula_kda_bwd_gated_checked) X(cula_kda_clear) X(cula_kda_gate_fwd) X(cula_kda_gate_bwd)                              \
     X(cula_kda_beta_sigmoid_fwd) X(cula_kda_beta_sigmoid_bwd) X(cula_kda_short_conv_fwd) X(cula_kda_short_conv_bwd)    \
     X(cula_kda_rms_norm_gated_fwd) X(cula_kda_rms_norm_gated_bwd) X(cula_kda_strerror)                         \
-    X(cula_kda_selective_scan_fwd) X(cula_kda_selective_scan_bwd) X(cula_kda_selective_scan_tiles) X(cula_kda_selective_step)            \
+    X(cula_kda_selective_scan_fwd) X(cula_kda_selective_scan_bwd) X(cula_kda_selective_scan_tiles) X(cula_kda_selective_scan_state_floats) X(cula_kda_selective_step)            \
     X(cula_kda_conv_step) X(cula_kda_add_rms_norm_fwd) X(cula_kda_add_rms_norm_bwd) X(cula_kda_add_rms_norm_shares)
 struct Lib {
 #define CULA_KDA_MEMBER(name) decltype(&::name) name = nullptr;

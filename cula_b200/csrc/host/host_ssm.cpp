@@ -122,7 +122,7 @@ ScanOutputs scan_forward(const ScanInputs& in, bool want_final, bool keep) {
     if (in.tab && in.tab->total_tokens < s.T) o.y.narrow(1, in.tab->total_tokens, s.T - in.tab->total_tokens).zero_();      // rows past the packed tokens
     if (want_final) o.hT = device_empty({s.n_seqs, s.D, s.S}, f32);
     if (keep) {
-        o.states = device_empty({s.num_chunks * (CHUNK / KEEP), s.D, s.SP}, f32);
+        o.states = device_empty({s.num_chunks * (CHUNK / KEEP), lib.cula_kda_selective_scan_state_floats((int)s.D, (int)s.G, (int)s.S)}, f32);
         if (has(in.z)) o.y_pre = device_empty({s.B, s.T, s.D}, f32);
     }
     cula_kda_selective_scan_args a = scan_args(in, s);

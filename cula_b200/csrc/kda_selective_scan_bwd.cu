@@ -16,6 +16,22 @@ constexpr int SEL_SCAN_REGS = 184, SEL_SERVE_REGS = 72;             // of a thre
 
 __device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(SEL_BWD_THREADS) : "memory"); }
 
+// Sums over the channels of a warp for gradients in 16 bits (dB, dC) go over neighbouring lanes by matrix instructions that multiply with
+// ones: 2 of them and 4 other instructions per token instead of 28, 7 of which are exchanges through shared memory's data path, which
+// bounds this kernel. The instruction drops all but 10 bits behind the leading one of a thread's value (two channels' sum; further sums are
+// fp32): independent errors of at most 2^-10 of a term, against the 2^-8 of the result's own rounding. Their mean, 2^-11 (1 - 1/2) / ln 2 for
+// evenly spread exponents, is put back at the end. 16 lanes over states leave too few neighbours over channels.
+template <int SL, typename T>
+constexpr bool sel_tensor_sums() { return sizeof(T) == 2 && SL <= 8; }
+constexpr float SEL_DROPPED = 1.f + 0.7213475f / 2048.f;
+// c += what (a0, a2) are over four neighbouring lanes, in the columns that b0, b1 mark; likewise (a1, a3) eight rows below
+__device__ __forceinline__ void sel_sum4(float (&c)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)),
+          "r"(__float_as_uint(b1)));
+}
+
 template <int SL, typename T>
 struct SelBwdSmem {
     using G = SelShape<SL>;
@@ -25,16 +41,20 @@ struct SelBwdSmem {
     float4 b[2][G::LC][SL], c[2][G::LC][SL];
     float4 sums[2][G::LC][G::CH / 2];                                // two channels' sum_n g B, sum_n w A (log2 units)
     float bc[2][SEL_WARPS][G::LC][2 * G::SP];                        // per warp: dB, dC
-    float par[2][G::CH];                                             // dt_bias, skip
+    float2 par[2][4][G::VECS];                                       // dt_bias, skip: [which][pair of a piece][piece]
     T raw_b[RING][G::UNITS][4], raw_c[RING][G::UNITS][4];            // B and C rows as they are
     uint4 raw[RING][4][Q][G::ITEMS];                                 // x, dt, z, dout rows as they are
-    float4 kept[G::LC / SEL_KEEP][2][SEL_THREADS];                   // each thread's states before every eighth token
-    float4 acc[4][G::ITEMS];                                         // a thread's sums for dskip and dbias (8 channels each)
+    union {
+        float4 kept[G::LC / SEL_KEEP][2][SEL_THREADS];               // each thread's states before every eighth token
+        float4 acc[4][G::ITEMS];                                     // at the end: the serving threads' sums for dskip and dbias
+    };
+    static_assert(sizeof(acc) <= 2 * sizeof(kept), "");
 };
 
 // What the serving warps do for an item: rows of the tiles to come, operands of the next tile, gradients of the one before.
 template <int SL, typename T, bool STATE_ONLY>
-__device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<SL, T>& sm, const SelItem& it, int d0, int d_end, int group, int share) {
+__device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<SL, T>& sm, const SelItem& it, int d0, int d_end, int group, int share,
+                                              float2 (&acc)[2][4]) {
     using G = SelShape<SL>;
     using V = SelVec<T>;
     constexpr int LC = G::LC, SP = G::SP, Q = V::Q, RING = SelBwdSmem<SL, T>::RING;
@@ -49,7 +69,6 @@ __device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<S
     const T* bp = static_cast<const T*>(a.Bm) + batch * a.b_seq + first * a.b_row + group * a.S;
     const T* cp = static_cast<const T*>(a.Cm) + batch * a.c_seq + first * a.c_row + group * a.S;
     const int x_row = (int)a.x_row, dt_row = (int)a.dt_row, z_row = (int)a.z_row, b_row = (int)a.b_row, c_row = (int)a.c_row;
-    auto param = [&](int which, float2 (&v)[4]) { SelVec<float>::unpack(reinterpret_cast<const uint4*>(&sm.par[which][8 * vec]), 1, v); };
     // tiles are taken from the last to the first; the j-th taken is tile n_tiles - 1 - j
     auto fetch = [&](int j) {
         const int t_first = it.t0 + (n_tiles - 1 - j) * LC, t = t_first + tt, slot = j % RING;
@@ -78,11 +97,10 @@ __device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<S
         if (tid < G::ITEMS) {                                        // zeros for channels past the tile: they add nothing to dB and dC
             const bool live = item && t_first + tt < it.t1;
             const uint4(*from)[Q][G::ITEMS] = sm.raw[slot];
-            float2 x[4], d[4], b[4];
+            float2 x[4], d[4];
             V::unpack(&from[1][0][tid], G::ITEMS, d);
-            param(0, b);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = add2(d[e], b[e]);
+            for (int e = 0; e < 4; ++e) d[e] = add2(d[e], sm.par[0][e][vec]);
             if (a.softplus) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = sel_softplus2(d[e]);
@@ -131,38 +149,20 @@ __device__ __forceinline__ void sel_bwd_serve(const SelScanArgs& a, SelBwdSmem<S
             float2 x[4], d[4], sg[4];
             V::unpack(&from[1][0][tid], G::ITEMS, d);
             if (a.softplus) {
-                float2 b[4];
-                param(0, b);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sg[e] = sel_sigmoid2(add2(d[e], b[e]));
+                for (int e = 0; e < 4; ++e) sg[e] = sel_sigmoid2(add2(d[e], sm.par[0][e][vec]));
             } else sg[0] = sg[1] = sg[2] = sg[3] = splat2(1.f);
             V::unpack(&from[0][0][tid], G::ITEMS, x);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float4 sums = sm.sums[buf][tt][e * G::VECS + vec];
-                d[e] = mul2(fma2(x[e], make_float2(sums.x, sums.z), mul2(make_float2(sums.y, sums.w), splat2(0.6931471805599453f))), sg[e]);      // A is held times log2(e)
+                const float4 sums = sm.sums[buf][tt][e * G::VECS + vec], step = sm.dx[buf][tt][e * G::VECS + vec];
+                const float2 gB = make_float2(sums.x, sums.z), dy = sm.dy[buf][tt][e * G::VECS + vec];
+                d[e] = mul2(fma2(x[e], gB, mul2(make_float2(sums.y, sums.w), splat2(0.6931471805599453f))), sg[e]);      // A is held times log2(e)
+                acc[0][e] = fma2(dy, x[e], acc[0][e]);
+                acc[1][e] = add2(acc[1][e], d[e]);
+                x[e] = fma2(make_float2(step.x, step.y), gB, mul2(sm.par[1][e][vec], dy));
             }
             V::store(static_cast<T*>(a.ddt) + at, d);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float4 ab = sm.acc[2 + h][tid];
-                ab.x += d[2 * h].x; ab.y += d[2 * h].y; ab.z += d[2 * h + 1].x; ab.w += d[2 * h + 1].y;
-                sm.acc[2 + h][tid] = ab;
-            }
-            param(1, d);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float4 as = sm.acc[h][tid];
-#pragma unroll
-                for (int e = 2 * h; e < 2 * h + 2; ++e) {
-                    const float4 step = sm.dx[buf][tt][e * G::VECS + vec], sums = sm.sums[buf][tt][e * G::VECS + vec];
-                    const float2 dy = sm.dy[buf][tt][e * G::VECS + vec], ds = mul2(dy, x[e]);
-                    if (e & 1) { as.z += ds.x; as.w += ds.y; }
-                    else { as.x += ds.x; as.y += ds.y; }
-                    x[e] = fma2(make_float2(step.x, step.y), make_float2(sums.x, sums.z), mul2(d[e], dy));
-                }
-                sm.acc[h][tid] = as;
-            }
             V::store(static_cast<T*>(a.dx) + at, x);
             if (gate) {
                 float2 z[4], o[4];
@@ -227,20 +227,25 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         // Of the 128 registers per thread that the block starts with, the serving warps give up what the scanning ones need
         if constexpr (!STATE_ONLY) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(SEL_SERVE_REGS));
         for (int i = tid; i < CH; i += SEL_THREADS) {
-            sm.par[0][i] = a.dt_bias && d0 + i < d_end ? a.dt_bias[d0 + i] : 0.f;
-            sm.par[1][i] = a.skip && d0 + i < d_end ? a.skip[d0 + i] : 0.f;
-        }
-        if (!STATE_ONLY && tid < G::ITEMS) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const bool in = d0 + i < d_end;
+            (&sm.par[0][i / 2 % 4][i / 8].x)[i & 1] = in && a.dt_bias ? a.dt_bias[d0 + i] : 0.f;
+            (&sm.par[1][i / 2 % 4][i / 8].x)[i & 1] = in && a.skip ? a.skip[d0 + i] : 0.f;
         }
         asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
+        float2 acc[2][4];                                            // dskip and dbias of the thread's 8 channels
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][e] = acc[1][e] = make_float2(0.f, 0.f);
         for (long long i = row; i < items; i += a.cta_rows) {
             SelItem it;
             if (!sel_item(a, i, it) || (STATE_ONLY && it.seg == 0)) continue;
-            sel_bwd_serve<SL, T, STATE_ONLY>(a, sm, it, d0, d_end, group, share);
+            sel_bwd_serve<SL, T, STATE_ONLY>(a, sm, it, d0, d_end, group, share, acc);
         }
         if constexpr (!STATE_ONLY) {
+            sel_bwd_barrier();                                       // the scanning warps have read their last states
+            if (tid < G::ITEMS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sm.acc[e][tid] = make_float4(acc[e / 2][2 * (e & 1)].x, acc[e / 2][2 * (e & 1)].y, acc[e / 2][2 * (e & 1) + 1].x, acc[e / 2][2 * (e & 1) + 1].y);
+            }
             asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
             // dskip and dbias: the threads that stood at the same channels, in order
             for (int i = tid; i < 4 * G::VECS; i += SEL_THREADS) {
@@ -273,6 +278,11 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         }
     }
 
+    constexpr bool TENSOR = !STATE_ONLY && sel_tensor_sums<SL, T>();
+    float ones[8];                                                   // columns of the sums on tensor cores
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ones[k] = (lane >> 2) == k ? 1.f : 0.f;
+
     for (long long i = row; i < items; i += a.cta_rows) {
         SelItem it;
         if (!sel_item(a, i, it) || (STATE_ONLY && it.seg == 0)) continue;        // nothing comes before a first segment
@@ -280,10 +290,10 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         // the kept states of place `sub` of the j-th tile taken
         auto fetch = [&](int j, int sub) {
             const int at = it.t0 + (n_tiles - 1 - j) * LC + sub * KEEP;
-            if (own && j < n_tiles && at < it.t1) {
-                const float* from = a.states + ((size_t)(it.chunk0 * (BT / KEEP) + at / KEEP) * a.D + dc) * SP + n0;
+            if (j < n_tiles && at < it.t1) {
+                const float4* from = sel_kept<SL>(a, it.chunk0, at, tile, tiles) + warp * 64 + lane;
                 sel_copy16(&sm.kept[sub][0][tid], from);
-                sel_copy16(&sm.kept[sub][1][tid], from + SP);
+                sel_copy16(&sm.kept[sub][1][tid], from + 32);
             }
             sel_commit();
         };
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                     sel_wait<SUBS - 1>();
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float4 r = own ? sm.kept[sub][c][tid] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float4 r = sm.kept[sub][c][tid];
                         st[0][c][0] = make_float2(r.x, r.y);
                         st[0][c][1] = make_float2(r.z, r.w);
                     }
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                         }
                     }
                     constexpr int TB = SL > 4 ? SL / 4 : 1;          // tokens whose sums over states are added up together
-                    float v[4 * TB];
+                    float v[4 * TB], bc[4];
                     // the next token's rows are asked for before this one's sums are stored: no load waits behind a store
                     float4 dx_n = sm.dx[buf][tb + KEEP - 1][pair], b_n = sm.b[buf][tb + KEEP - 1][s], c_n = sm.c[buf][tb + KEEP - 1][s];
                     float2 dy_n = sm.dy[buf][tb + KEEP - 1][pair];
@@ -405,20 +415,39 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                                 reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][pair])[2 * ch + which] = r[k];
                             }
                         }
-                        float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
-                        sel_reduce<8, CL>(r, lane, 1);
-                        if constexpr (CL >= 8) {
-                            constexpr int REP = CL / 8;              // lanes left with the same value
-                            if (REP == 1 || cl % REP == 0) {
-                                const int id = cl / REP;
-                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
+                        if constexpr (TENSOR) {
+                            // columns of the token of two: states n0..n0+3; rows: dB and (below) dC of the lanes' quads
+                            const int w = 4 * (u & 1);
+                            if (u & 1) bc[0] = bc[1] = bc[2] = bc[3] = 0.f;
+                            sel_sum4(bc, dB0.x, dC0.x, dB0.y, dC0.y, ones[w], ones[w + 1]);
+                            sel_sum4(bc, dB1.x, dC1.x, dB1.y, dC1.y, ones[w + 2], ones[w + 3]);
+                            if (!(u & 1)) {
+                                constexpr int HI = CL / 4, LEFT = 4 / HI;        // quads of lanes over channels, values that each lane is left with
+                                sel_reduce<4, HI>(bc, lane, 4);
+                                float* to = sm.bc[buf][warp][tb + u + ((lane >> 1) & 1)] + n0 + 2 * (lane & 1);
+#pragma unroll
+                                for (int k = 0; k < LEFT; k += LEFT > 1 ? 2 : 1) {
+                                    const int id = (cl >> 2) * LEFT + k;
+                                    if constexpr (LEFT > 1) *reinterpret_cast<float2*>(to + (id >> 1) * SP) = make_float2(bc[k], bc[k + 1]);
+                                    else to[(id >> 1) * SP + (id & 1)] = bc[k];
+                                }
                             }
                         } else {
-                            constexpr int LEFT = 8 / CL;
+                            float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
+                            sel_reduce<8, CL>(r, lane, 1);
+                            if constexpr (CL >= 8) {
+                                constexpr int REP = CL / 8;          // lanes left with the same value
+                                if (REP == 1 || cl % REP == 0) {
+                                    const int id = cl / REP;
+                                    sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
+                                }
+                            } else {
+                                constexpr int LEFT = 8 / CL;
 #pragma unroll
-                            for (int k = 0; k < LEFT; ++k) {
-                                const int id = cl * LEFT + k;
-                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
+                                for (int k = 0; k < LEFT; ++k) {
+                                    const int id = cl * LEFT + k;
+                                    sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
+                                }
                             }
                         }
                     }
@@ -441,6 +470,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         }
     }
     if constexpr (!STATE_ONLY) {
+        sel_bwd_barrier();
         if (own) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -451,7 +481,8 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
 
 // ---- the shares added up: dB and dC (one thread per token row, group and four states), then dA, dskip, dbias (one per value) ----
 template <typename T>
-__global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks) {
+__global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks,
+                                                                    const float scale) {
     pdl_launch_dependents();
     pdl_wait();
     if (blockIdx.x < bc_blocks) {
@@ -467,7 +498,7 @@ __global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelSc
             }
         }
         T* to = static_cast<T*>(isC ? a.dCm : a.dBm) + rg * a.S;
-        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        const float f[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (n + k < a.S) {
@@ -520,7 +551,8 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
         return (int)e;
     const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 255) / 256, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
     if (bc_blocks + rest > 0x7fffffffLL) return -1;
-    return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks);
+    return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks,
+                             sel_tensor_sums<SL, T>() ? SEL_DROPPED : 1.f);
 }
 
 }  // namespace kda

@@ -18,7 +18,7 @@ struct SelFwdSmem {
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float4 b[2][G::LC][G::SL], c[2][G::LC][G::SL];
     float2 y[2][G::LC][G::CH / 2 + 2];                               // rows shifted against each other: no bank conflicts of the writers
-    float par[2][G::CH];                                             // dt_bias, skip
+    float2 par[2][4][G::VECS];                                       // dt_bias, skip: [which][pair of a piece][piece]
     T raw_b[SEL_AHEAD][G::UNITS][4], raw_c[SEL_AHEAD][G::UNITS][4];                  // B and C rows as they are
     uint4 raw[SEL_AHEAD][3][Q][G::ITEMS];                                    // x, dt, z rows as they are: [stage][which][piece][thread]
 };
@@ -79,11 +79,15 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
             sel_commit();
         };
         for (int i = tid; i < CH; i += SEL_THREADS) {
-            sm.par[0][i] = a.dt_bias && d0 + i < d_end ? a.dt_bias[d0 + i] : 0.f;
-            sm.par[1][i] = a.skip && d0 + i < d_end ? a.skip[d0 + i] : 0.f;
+            const bool in = d0 + i < d_end;
+            (&sm.par[0][i / 2 % 4][i / 8].x)[i & 1] = in && a.dt_bias ? a.dt_bias[d0 + i] : 0.f;
+            (&sm.par[1][i / 2 % 4][i / 8].x)[i & 1] = in && a.skip ? a.skip[d0 + i] : 0.f;
         }
         asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
-        auto param = [&](int which, float2 (&v)[4]) { SelVec<float>::unpack(reinterpret_cast<const uint4*>(&sm.par[which][dv - d0]), 1, v); };
+        auto param = [&](int which, float2 (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = sm.par[which][e][tid % G::VECS];
+        };
         auto stage = [&](int k) {                                        // tile k, arrived, as the scan takes it; zeros past the end change no state
             const int buf = k & 1, slot = k % SEL_AHEAD;
             if (tid < G::ITEMS) {
@@ -202,10 +206,10 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
         float v[2 * LC];
 #pragma unroll
         for (int u = 0; u < LC; ++u) {
-            if (!STATE_ONLY && u % SEL_KEEP == 0 && a.states && own && it.t0 + k * LC + u < it.t1) {
-                float* to = a.states + ((size_t)(it.chunk0 * (BT / SEL_KEEP) + (it.t0 + k * LC + u) / SEL_KEEP) * a.D + dc) * SP + n0;
+            if (!STATE_ONLY && u % SEL_KEEP == 0 && a.states && it.t0 + k * LC + u < it.t1) {
+                float4* to = sel_kept<SL>(a, it.chunk0, it.t0 + k * LC + u, tile, tiles) + warp * 64 + lane;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) *reinterpret_cast<float4*>(to + c * SP) = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
+                for (int c = 0; c < 2; ++c) to[c * 32] = make_float4(h[c][0].x, h[c][0].y, h[c][1].x, h[c][1].y);
             }
             const float4 dx = sm.dx[buf][u][pair], b = sm.b[buf][u][s];
             if (STATE_ONLY) sum_dt = add2(sum_dt, make_float2(dx.x, dx.y));

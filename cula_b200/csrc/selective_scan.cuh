@@ -129,6 +129,12 @@ __device__ __forceinline__ void sel_fetch4(T* to, const T* row, int n, int S, in
         for (int k = 0; k < 4; ++k) to[k] = n + k < S ? row[n + k] : T(0.f);
     }
 }
+// Where the states that are kept for the backward pass stand: a thread's two times four of them as two 16-byte pieces, those of a warp in
+// order. Returned is the first piece of lane 0 of a CTA's warp 0; pieces follow as [warp][channel of two][lane].
+template <int SL>
+__device__ __forceinline__ float4* sel_kept(const SelScanArgs& a, long long chunk0, int t, int tile, int tiles) {
+    return reinterpret_cast<float4*>(a.states) + ((size_t)(chunk0 * (BT / SEL_KEEP) + t / SEL_KEEP) * tiles + tile) * (SEL_WARPS * 2 * 32);
+}
 // four states of a [.., S] fp32 row
 __device__ __forceinline__ void sel_load4(const float* row, int n, int S, float2 (&v)[2]) {
     float f[4];

@@ -329,7 +329,8 @@ typedef struct cula_kda_selective_scan_args {
     const float* h0;              /* [N, D, S] or NULL */
     void* y;                      /* [B*T, D]                                                                  (forward) */
     float* hT;                    /* [N, D, S] or NULL                                                         (forward) */
-    float* states;                /* [num_chunks * 8, D, SP]: the state before every eighth token; forward: NULL unless a backward pass follows */
+    float* states;                /* [num_chunks * 8, cula_kda_selective_scan_state_floats()]: the state before every eighth token, in the order of the
+                                     kernels' threads; forward: NULL unless a backward pass follows */
     float* y_pre;                 /* [B*T, D]: y before the gate, with z and `states` */
     const void* dy;               /* [B*T, D]                                                                  (backward from here) */
     const float* dhT;             /* [N, D, S] or NULL */
@@ -352,8 +353,9 @@ typedef struct cula_kda_selective_scan_args {
 } cula_kda_selective_scan_args;
 int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* args, void* stream);
 int cula_kda_selective_scan_bwd(const cula_kda_selective_scan_args* args, void* stream);
-/* channel tiles of a group, the first dimension of part_bc */
+/* channel tiles of a group, the first dimension of part_bc; floats of one kept state of all channels */
 int cula_kda_selective_scan_tiles(int D, int G, int S);
+int cula_kda_selective_scan_state_floats(int D, int G, int S);
 
 /* One token of that recurrence for each of `rows` sequences against a pool of states, updated in place. Negative slots skip a row (zero
  * output); slots past the pool do so too and set *status to 2. A slot may appear once in a call. */
