@@ -12,7 +12,7 @@
 namespace kda {
 
 constexpr int SEL_BWD_THREADS = 2 * SEL_THREADS;
-constexpr int SEL_SCAN_REGS = 184, SEL_SERVE_REGS = 72;             // of a thread of either kind; the block is launched with their mean
+constexpr int SEL_SCAN_REGS = 192, SEL_SERVE_REGS = 64;             // of a thread of either kind; the block is launched with their mean
 
 __device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(SEL_BWD_THREADS) : "memory"); }
 
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                             st[u + 1][c][1] = fma2(p, make_float2(b.z, b.w), mul2(av[u][c][1], st[u][c][1]));
                         }
                     }
-                    constexpr int TB = SL > 4 ? SL / 4 : 1;          // tokens whose sums over states are added up together
+                    constexpr int TB = SL > 4 ? SL / 4 : 2;          // tokens whose sums over states are added up together
                     float v[4 * TB], bc[4];
                     // the next token's rows are asked for before this one's sums are stored: no load waits behind a store
                     float4 dx_n = sm.dx[buf][tb + KEEP - 1][pair], b_n = sm.b[buf][tb + KEEP - 1][s], c_n = sm.c[buf][tb + KEEP - 1][s];
@@ -407,13 +407,12 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
 #pragma unroll
                             for (int k = 0; k < 4 * TB; ++k) r[k] = v[k];
                             sel_reduce<4 * TB, SL>(r, lane, CL);
-                            constexpr int LEFT = 4 * TB / SL;        // 1, or 2 where two lanes share four values
-                            const int at = s * LEFT;
-#pragma unroll
-                            for (int k = 0; k < LEFT; ++k) {
-                                const int id = at + k, tok = id / 4, ch = (id >> 1) & 1, which = id & 1;
-                                reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][pair])[2 * ch + which] = r[k];
-                            }
+                            constexpr int LEFT = 4 * TB / SL;        // values that each lane is left with
+                            const int tok = s * LEFT / 4, at = s * LEFT % 4;
+                            float* to = reinterpret_cast<float*>(&sm.sums[buf][tb + u + tok][pair]) + at;
+                            if constexpr (LEFT == 4) *reinterpret_cast<float4*>(to) = make_float4(r[0], r[1], r[2], r[3]);
+                            else if constexpr (LEFT == 2) *reinterpret_cast<float2*>(to) = make_float2(r[0], r[1]);
+                            else *to = r[0];
                         }
                         if constexpr (TENSOR) {
                             // columns of the token of two: states n0..n0+3; rows: dB and (below) dC of the lanes' quads
