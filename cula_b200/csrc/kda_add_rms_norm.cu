@@ -82,18 +82,22 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
     for (int v = 0; v < VPT; ++v)
         if (const int c = lane + v * TPR; c < nv) w[v].load(a.w + 8 * c);
     int parity = 0;
-    for (long long row = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR; row - threadIdx.x / TPR < a.R; row += (long long)gridDim.x * GROUPS, parity ^= 1) {
-        const bool live = row < a.R;
-        Oct<T> rx[VPT];
-        Oct<R> rr[VPT];
+    Oct<T> rx[VPT];
+    Oct<R> rr[VPT];
+    auto fetch = [&](long long row) {
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = lane + v * TPR;
-            if (live && c < nv) {
+            if (row < a.R && c < nv) {
                 rx[v].load(static_cast<const T*>(a.x) + row * a.x_row + 8 * c);
                 if (RES != RES_NONE) rr[v].load(static_cast<const R*>(a.r) + row * a.r_row + 8 * c);
             }
         }
+    };
+    const long long row0 = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR, step = (long long)gridDim.x * GROUPS;
+    fetch(row0);
+    for (long long row = row0; row - threadIdx.x / TPR < a.R; row += step, parity ^= 1) {
+        const bool live = row < a.R;
         float2 val[VPT][4], ss = make_float2(0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -113,6 +117,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
                 for (int e = 0; e < 4; ++e) ss = fma2(val[v][e], val[v][e], ss);
             }
         }
+        fetch(row + step);                                           // on its way while this row is summed, scaled and stored
         const float rstd = rsqrtf(row_sum<TPR>(ss.x + ss.y, s_sum[parity]) * (1.f / a.D) + a.eps);
         if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
         int top = 0;                                                 // bits of the largest |y|: a NaN is larger than anything
@@ -192,21 +197,27 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_bwd_ker
         if (c < nv) w[v].load(a.w + 8 * c);
     }
     int parity = 0;
-    for (long long row = group; row - threadIdx.x / TPR < a.R; row += (long long)gridDim.x * GROUPS, parity ^= 1) {
-        const bool live = row < a.R;
-        Oct<R> rv[VPT], rd[VPT];
-        Oct<T> ry[VPT];
-        const float rstd = live ? a.rstd[row] : 0.f;
+    Oct<R> rv[VPT], rd[VPT], cd[VPT];
+    Oct<T> ry[VPT];
+    float next_rstd = 0.f;
+    auto fetch = [&](long long row) {
+        if (row < a.R) next_rstd = a.rstd[row];
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = lane + v * TPR;
-            if (live && c < nv) {
+            if (row < a.R && c < nv) {
                 const size_t at = (size_t)row * a.D + 8 * c;
                 rv[v].load(static_cast<const R*>(a.v) + (RES == RES_NONE ? row * a.x_row + 8 * c : at));
                 ry[v].load(static_cast<const T*>(a.dy) + at);
                 if (RES != RES_NONE && a.dr_out) rd[v].load(static_cast<const R*>(a.dr_out) + at);
             }
         }
+    };
+    const long long step = (long long)gridDim.x * GROUPS;
+    fetch(group);
+    for (long long row = group; row - threadIdx.x / TPR < a.R; row += step, parity ^= 1) {
+        const bool live = row < a.R;
+        const float rstd = next_rstd;
         float2 n[VPT][4], dn[VPT][4], dot = make_float2(0.f, 0.f);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -226,6 +237,9 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_bwd_ker
                 }
             }
         }
+#pragma unroll
+        for (int v = 0; v < VPT; ++v) cd[v] = rd[v];
+        fetch(row + step);                                           // on its way while this row is summed and stored
         const float m = -row_sum<TPR>(dot.x + dot.y, s_sum[parity]) * (1.f / a.D);
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_bwd_ker
             if (live && c < nv) {
                 const size_t at = (size_t)row * a.D + 8 * c;
                 float2 dv[4], d[4];
-                if (RES != RES_NONE && a.dr_out) rd[v].get(d);
+                if (RES != RES_NONE && a.dr_out) cd[v].get(d);
                 else d[0] = d[1] = d[2] = d[3] = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) dv[e] = fma2(splat2(rstd), fma2(n[v][e], splat2(m), dn[v][e]), d[e]);
@@ -259,24 +273,23 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_bwd_ker
     }
 }
 
-// the shares of dw added up in a fixed order: 32 columns per block, eight threads to a column
-__global__ void __launch_bounds__(256) kda_add_rms_norm_sum_kernel(const float* part, float* dw, int D, int rows) {
-    __shared__ float s[8][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), k0 = threadIdx.x >> 5;
+// the shares of dw added up in a fixed order: 32 columns per block, 32 threads to a column
+__global__ void __launch_bounds__(1024) kda_add_rms_norm_sum_kernel(const float* part, float* dw, int D, int rows) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, k0 = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
     pdl_launch_dependents();
     pdl_wait();
     float sum = 0.f;
     if (col < D) {
 #pragma unroll 8
-        for (int k = k0; k < rows; k += 8) sum += part[(size_t)k * D + col];
+        for (int k = k0; k < rows; k += 32) sum += part[(size_t)k * D + col];
     }
-    s[k0][threadIdx.x & 31] = sum;
+    s[k0][lane] = sum;
     __syncthreads();
-    if (k0 == 0 && col < D) {
+    sum = s[lane][k0];                                               // a warp per column
 #pragma unroll
-        for (int k = 1; k < 8; ++k) sum += s[k][threadIdx.x];
-        dw[col] = sum;
-    }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0 && blockIdx.x * 32 + k0 < D) dw[blockIdx.x * 32 + k0] = sum;
 }
 
 // Threads and pieces for a row: a warp up to 1024 columns, two pieces per thread above that. Where rows are few, one piece per thread
@@ -323,7 +336,7 @@ static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
     const int threads = norm_threads(s.tpr), groups = threads / s.tpr;
     const long long blocks = norm_bwd_blocks(a.D, a.R, s);
     if (const cudaError_t e = launch_early(kernel, dim3((unsigned)blocks), threads, 0, stream, a); e != cudaSuccess) return (int)e;
-    return (int)launch_early(kda_add_rms_norm_sum_kernel, dim3((a.D + 31) / 32), 256, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)(blocks * groups));
+    return (int)launch_early(kda_add_rms_norm_sum_kernel, dim3((a.D + 31) / 32), 1024, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)(blocks * groups));
 }
 
 }  // namespace kda

@@ -478,23 +478,33 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
     }
 }
 
-// ---- the shares added up: dB and dC (one thread per token row, group and four states), then dA, dskip, dbias (one per value) ----
+// ---- the shares added up: dB and dC (four threads per token row, group and four states, one after the other's part of the shares), then dA,
+//      dskip, dbias (one thread per value) ----
 template <typename T>
 __global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks,
                                                                     const float scale) {
+    __shared__ float4 part[3][64];
     pdl_launch_dependents();
     pdl_wait();
     if (blockIdx.x < bc_blocks) {
-        const long long i = (long long)blockIdx.x * 256 + threadIdx.x, quads = SP / 2, rg = i / quads;
-        if (rg >= a.rows * a.G) return;
+        const int me = threadIdx.x & 63, quarter = threadIdx.x >> 6, per = (tiles_per_group + 3) / 4;
+        const long long i = (long long)blockIdx.x * 64 + me, quads = SP / 2, rg = i / quads;
         const int q = (int)(i - rg * quads), isC = q >= SP / 4, n = 4 * (q % (SP / 4));
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!a.cu_seqlens || rg / a.G < a.total_tokens) {            // rows past the packed tokens have zero gradients
+        if (rg < a.rows * a.G && (!a.cu_seqlens || rg / a.G < a.total_tokens)) {       // rows past the packed tokens have zero gradients
 #pragma unroll 8
-            for (int k = 0; k < tiles_per_group; ++k) {
+            for (int k = quarter * per; k < min(tiles_per_group, (quarter + 1) * per); ++k) {
                 const float4 r = *reinterpret_cast<const float4*>(a.part_bc + ((size_t)k * a.rows * a.G + rg) * (2 * SP) + 4 * q);
                 sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
             }
+        }
+        if (quarter) part[quarter - 1][me] = sum;
+        __syncthreads();
+        if (quarter || rg >= a.rows * a.G) return;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const float4 r = part[k][me];
+            sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
         }
         T* to = static_cast<T*>(isC ? a.dCm : a.dBm) + rg * a.S;
         const float f[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
@@ -512,7 +522,7 @@ __global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelSc
         if (i >= nA + 2LL * a.D) return;
         if ((i >= nA && i < nA + a.D && !a.dskip) || (i >= nA + a.D && !a.dbias)) return;
         float sum = 0.f;
-#pragma unroll 4
+#pragma unroll 8
         for (int k = 0; k < a.cta_rows; ++k) sum += from[k * stride];
         if (i < nA) {
             const int n = (int)(i % SP);
@@ -548,7 +558,7 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
     if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_BWD_THREADS, smem, stream, a, tpg, items);
         e != cudaSuccess)
         return (int)e;
-    const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 255) / 256, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
+    const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 63) / 64, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
     if (bc_blocks + rest > 0x7fffffffLL) return -1;
     return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks,
                              sel_tensor_sums<SL, T>() ? SEL_DROPPED : 1.f);
