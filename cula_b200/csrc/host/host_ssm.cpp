@@ -1,4 +1,5 @@
 // The operators of a selective state space block (selective scan, single-token steps, residual RMS norm) on the native host path.
+#include <algorithm>
 #include <climits>
 
 #include "host_common.h"
@@ -11,7 +12,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 constexpr int64_t KEEP = 8;                    // tokens per kept state
-constexpr int64_t SMS = 148, CTAS_PER_SM = 2;  // two CTAs of the scan per SM come near its throughput
+constexpr int64_t SMS = 148;
 
 bool grad_wanted(std::initializer_list<OptTensor> ts) {
     for (const OptTensor& t : ts)
@@ -78,13 +79,32 @@ ScanSizes sizes_of(const ScanInputs& in) {
     s.tiles = lib.cula_kda_selective_scan_tiles((int)s.D, (int)s.G, (int)s.S) * s.G;
     return s;
 }
+// Microseconds that CTAs take for a 64-token chunk of a tile of channels (16 states): one alone on its SM, and two that share it
+struct ScanCost { double alone, shared; };
+double scan_time(double ctas, double chunks, ScanCost c) {
+    const double set_up = 3.5;                                       // parameters, the first rows
+    if (ctas <= SMS) return set_up + chunks * c.alone;
+    const double one = set_up + chunks * c.shared;
+    return ctas <= 2 * SMS ? one : one * (ctas / (2 * SMS) + 0.5);  // the last ones are half as long behind the rest on average
+}
 // Chunks per segment, 0 for sequences in one piece. Cutting takes a launch more, which makes the exponentials of nearly all tokens once
-// more (`extra` of the whole work), and pays where the longest sequence would keep the call waiting for longer than that.
-int64_t plan_segments(const ScanSizes& s, double extra) {
-    const double slots = double(SMS * CTAS_PER_SM), work = double(s.num_chunks) * s.tiles / slots;      // chunks per slot
-    if (s.longest < 8 || double(s.longest) < (1.0 + extra) * work + 6.0) return 0;
-    const int64_t seg = std::max<int64_t>(2, (int64_t)std::ceil(work));
-    return seg < s.longest ? seg : 0;
+// more, and pays where few or long sequences would leave SMs waiting. Measured on both sides: 4 x 2048 x 4096 channels (256 CTAs) forward
+// 229 us whole; 1 x 4096 x 4096 (64 CTAs) 270 whole, 190 cut; 2 x 333 x 528 (20 CTAs) forward 30 whole, backward 70.
+int64_t plan_segments(const ScanSizes& s, bool backward) {
+    const ScanCost walk = backward ? ScanCost{11.3, 17.7} : ScanCost{4.3, 7.0}, first = backward ? ScanCost{4.0, 5.2} : ScanCost{3.0, 5.2};
+    const double total = (double)s.num_chunks, tiles = (double)s.tiles;
+    double best = std::max(scan_time((double)s.n_seqs * tiles, total / (double)std::max<int64_t>(1, s.n_seqs), walk), (double)s.longest * walk.alone);
+    int64_t seg = 0;
+    for (int64_t k = 1; k < s.longest; k += (k + 3) / 4) {
+        const double ctas = tiles * (s.num_chunks / (double)k + 0.5 * (double)s.n_seqs);       // sequences are not whole segments
+        const double folded = 0.2 * (double)(s.longest / k);        // a segment takes in the ones before it
+        const double time = scan_time(ctas, (double)k, walk) + scan_time(ctas, (double)k, first) + 4.0 + folded;
+        if (time < 0.95 * best) {
+            best = time;
+            seg = k;
+        }
+    }
+    return seg;
 }
 int64_t segment_slots(const ScanSizes& s, const ScanInputs& in, int64_t seg) {
     if (!seg) return 0;
@@ -195,7 +215,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         a.seg_chunks = (int)plan_segments(s, 0.5);
         const int64_t n_seg = segment_slots(s, in, a.seg_chunks);
         const int64_t items = a.seg_chunks ? n_seg : s.n_seqs;
-        a.cta_rows = (int)std::max<int64_t>(1, std::min(items, 4 * SMS * CTAS_PER_SM / s.tiles));
+        a.cta_rows = (int)std::max<int64_t>(1, std::min(items, 8 * SMS / s.tiles));
         // one workspace: shares of dB and dC, of dA, dskip and dbias, segments
         const int64_t n_bc = s.tiles / s.G * a.rows * s.G * 2 * s.SP, n_A = a.cta_rows * s.D * (s.SP + 2);
         Tensor work = device_empty({n_bc + n_A + n_seg * s.D * (s.SP + 1)}, f32);

@@ -220,7 +220,6 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
     const int tiles = tiles_per_group * a.G, tile = blockIdx.x % tiles, row = blockIdx.x / tiles;
     const int group = tile / tiles_per_group, per_group = a.D / a.G, share = tile % tiles_per_group;
     const int d0 = group * per_group + share * CH, d_end = (group + 1) * per_group;
-    pdl_launch_dependents();
     pdl_wait();
 
     if (threadIdx.x >= SEL_THREADS) {
@@ -310,7 +309,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         }
         if constexpr (!STATE_ONLY) {
             if (own) {                                               // the segments after this one
-#pragma unroll 2
+#pragma unroll 4
                 for (int q = it.segs - 1; q > it.seg; --q) {
                     const size_t at = (size_t)(it.slot0 + q) * a.D + dc;
                     const float2 sum = *reinterpret_cast<const float2*>(a.seg_dt + at);
@@ -468,6 +467,8 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
             }
         }
     }
+    // Not before: what follows in the stream would take places beside CTAs that run for long, and leave other SMs empty.
+    pdl_launch_dependents();
     if constexpr (!STATE_ONLY) {
         sel_bwd_barrier();
         if (own) {
@@ -544,7 +545,7 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> done[2];
     if (a.seg_chunks) {
         if (const cudaError_t e = allow_smem(kda_selective_scan_bwd_kernel<SL, T, true>, smem, done[1]); e != cudaSuccess) return (int)launched(e);
-        if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, true>, dim3((unsigned)blocks), SEL_BWD_THREADS, smem, stream, a, tpg, items);
+        if (const cudaError_t e = sel_launch(sel_long(a), kda_selective_scan_bwd_kernel<SL, T, true>, blocks, SEL_BWD_THREADS, smem, stream, a, tpg, items);
             e != cudaSuccess)
             return (int)e;
     }
@@ -555,7 +556,7 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
         return cudaFuncGetAttributes(&f, kda_selective_scan_bwd_kernel<SL, T, false>) == cudaSuccess && 2 * f.numRegs >= SEL_SCAN_REGS + SEL_SERVE_REGS;
     }();
     if (!enough) return (int)cudaErrorLaunchOutOfResources;
-    if (const cudaError_t e = launch_early(kda_selective_scan_bwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_BWD_THREADS, smem, stream, a, tpg, items);
+    if (const cudaError_t e = sel_launch(sel_long(a), kda_selective_scan_bwd_kernel<SL, T, false>, blocks, SEL_BWD_THREADS, smem, stream, a, tpg, items);
         e != cudaSuccess)
         return (int)e;
     const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 63) / 64, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;

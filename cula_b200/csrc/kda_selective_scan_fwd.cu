@@ -36,7 +36,6 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
     const int tiles = tiles_per_group * a.G, tile = blockIdx.x % tiles;
     const int group = tile / tiles_per_group, per_group = a.D / a.G;
     const int d0 = group * per_group + (tile % tiles_per_group) * CH, d_end = (group + 1) * per_group;
-    pdl_launch_dependents();
     pdl_wait();
     SelItem it;
     if (!sel_item(a, blockIdx.x / tiles, it)) return;
@@ -182,7 +181,7 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
     }
     if constexpr (!STATE_ONLY) {
         if (it.seg && own) {                                         // the segments before this one
-#pragma unroll 2
+#pragma unroll 4
             for (int q = 0; q < it.seg; ++q) {
                 const size_t at = (size_t)(it.slot0 + q) * a.D + dc;
                 const float2 sum = *reinterpret_cast<const float2*>(a.seg_dt + at);
@@ -234,6 +233,8 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
         }
         sel_barrier();
     }
+    // Not before: what follows in the stream would take places beside CTAs that run for long, and leave other SMs empty.
+    pdl_launch_dependents();
     if (!own) return;
     if constexpr (STATE_ONLY) {
         const size_t at = (size_t)(it.slot0 + it.seg) * a.D + dc;
@@ -260,12 +261,12 @@ static int launch_sel_fwd(const SelScanArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> done[2];
     if (a.seg_chunks) {
         if (const cudaError_t e = allow_smem(kda_selective_scan_fwd_kernel<SL, T, true>, smem, done[1]); e != cudaSuccess) return (int)launched(e);
-        if (const cudaError_t e = launch_early(kda_selective_scan_fwd_kernel<SL, T, true>, dim3((unsigned)blocks), SEL_FWD_THREADS, smem, stream, a, tpg);
+        if (const cudaError_t e = sel_launch(sel_long(a), kda_selective_scan_fwd_kernel<SL, T, true>, blocks, SEL_FWD_THREADS, smem, stream, a, tpg);
             e != cudaSuccess)
             return (int)e;
     }
     if (const cudaError_t e = allow_smem(kda_selective_scan_fwd_kernel<SL, T, false>, smem, done[0]); e != cudaSuccess) return (int)launched(e);
-    return (int)launch_early(kda_selective_scan_fwd_kernel<SL, T, false>, dim3((unsigned)blocks), SEL_FWD_THREADS, smem, stream, a, tpg);
+    return (int)sel_launch(sel_long(a), kda_selective_scan_fwd_kernel<SL, T, false>, blocks, SEL_FWD_THREADS, smem, stream, a, tpg);
 }
 
 }  // namespace kda

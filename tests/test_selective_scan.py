@@ -302,7 +302,11 @@ def test_a_prompt_in_two_calls(cut):
     y, fin = selective_scan(**d, output_final_state=True)
     y1, mid = selective_scan(**part(0, cut), output_final_state=True)
     y2, end = selective_scan(**part(cut, 150, initial_state=mid), output_final_state=True)
-    assert torch.equal(y, torch.cat([y1, y2], 1)) and torch.equal(fin, end)
+    # Not bit for bit: a sequence may be cut into segments, whose states are joined with one exponential of the sum of their steps in the
+    # place of a product of exponentials. Both are within 2^-22 per step of the definition (tol without the output's rounding), so they are
+    # within twice that of each other; outputs may then fall on either side of a rounding border, half a step of 2^-8 away.
+    assert err_ratio(fin.cpu(), end.cpu()) < 2 * tol(torch.float32, 150)
+    assert err_ratio(y.double().cpu(), torch.cat([y1, y2], 1).double().cpu()) < 2.0 ** -8 + 2 * tol(torch.float32, 150)
 
 
 @pytest.mark.gpu
