@@ -67,11 +67,13 @@ struct ScanInputs {
 };
 struct ScanSizes {
     int64_t B, T, D, S, G, SP, n_seqs, num_chunks, longest, tiles;        // longest: chunks of the longest sequence; tiles: of channels
+    bool packed;
 };
 ScanSizes sizes_of(const ScanInputs& in) {
     ScanSizes s{};
     s.B = in.x.size(0); s.T = in.x.size(1); s.D = in.x.size(2); s.G = in.B.size(2); s.S = in.B.size(3);
     s.SP = padded_states(s.S);
+    s.packed = in.tab.has_value();
     const int64_t cps = (s.T + CHUNK - 1) / CHUNK;
     s.n_seqs = in.tab ? in.tab->n_seqs : s.B;
     s.num_chunks = in.tab ? in.tab->num_chunks : s.B * cps;
@@ -79,26 +81,32 @@ ScanSizes sizes_of(const ScanInputs& in) {
     s.tiles = lib.cula_kda_selective_scan_tiles((int)s.D, (int)s.G, (int)s.S) * s.G;
     return s;
 }
-// Microseconds that CTAs take for a 64-token chunk of a tile of channels (16 states): one alone on its SM, and two that share it
+// Microseconds that a CTA takes for a 64-token chunk of a tile of channels (16 states): alone on its SM, and beside another one
 struct ScanCost { double alone, shared; };
-double scan_time(double ctas, double chunks, ScanCost c) {
-    const double set_up = 3.5;                                       // parameters, the first rows
-    if (ctas <= SMS) return set_up + chunks * c.alone;
-    const double one = set_up + chunks * c.shared;
-    return ctas <= 2 * SMS ? one : one * (ctas / (2 * SMS) + 0.5);  // the last ones are half as long behind the rest on average
+// and what that model of a launch lacks, fitted to sweeps over segments: setting up a CTA, the last CTAs' share, a segment taken in
+struct ScanFit { double set_up, tail, folded; };
+// of a launch of so many CTAs of at most so many chunks each, `work` chunks in all
+double scan_time(double ctas, double chunks, double work, ScanCost c, ScanFit f) {
+    const double places = 2.0 * SMS, one = f.set_up + chunks * (ctas <= SMS ? c.alone : c.shared);
+    return ctas <= places ? one : std::max(one, (work * c.shared + f.set_up * ctas) / places) + f.tail * one;
 }
 // Chunks per segment, 0 for sequences in one piece. Cutting takes a launch more, which makes the exponentials of nearly all tokens once
-// more, and pays where few or long sequences would leave SMs waiting. Measured on both sides: 4 x 2048 x 4096 channels (256 CTAs) forward
-// 229 us whole; 1 x 4096 x 4096 (64 CTAs) 270 whole, 190 cut; 2 x 333 x 528 (20 CTAs) forward 30 whole, backward 70.
+// more, and pays where few or long sequences would leave SMs waiting. Measured (whole, cut; us): 1 x 4096 tokens x 4096 channels forward
+// 266, 191, backward 725, 373; 1 x 16384 x 512 forward 1038, 115, backward 2775, 225; 2 x 4096 x 4096 forward 266, 358 (whole), 20 packed
+// sequences of 8192 in all x 2048 forward 152, 178 (whole), backward 549, 356; 1 x 512 x 4096 forward 39, 33.
 int64_t plan_segments(const ScanSizes& s, bool backward) {
     const ScanCost walk = backward ? ScanCost{11.3, 17.7} : ScanCost{4.3, 7.0}, first = backward ? ScanCost{4.0, 5.2} : ScanCost{3.0, 5.2};
-    const double total = (double)s.num_chunks, tiles = (double)s.tiles;
-    double best = std::max(scan_time((double)s.n_seqs * tiles, total / (double)std::max<int64_t>(1, s.n_seqs), walk), (double)s.longest * walk.alone);
+    const ScanFit fit = backward ? ScanFit{1.0, 0.25, 0.12} : ScanFit{2.0, 0.15, 0.03};
+    const double tiles = (double)s.tiles, work = (double)s.num_chunks * tiles, longest = (double)s.longest;
+    // whole: the longest sequence, beside others for as much of its time as there is work for the places beside it
+    const double beside = std::min(1.0, work / (2.0 * SMS * std::max(1.0, longest)));
+    double best = std::max((double)s.n_seqs * tiles <= SMS ? longest * walk.alone : longest * (walk.alone + beside * (walk.shared - walk.alone)),
+                           work * walk.shared / (2.0 * SMS));
     int64_t seg = 0;
     for (int64_t k = 1; k < s.longest; k += (k + 3) / 4) {
-        const double ctas = tiles * (s.num_chunks / (double)k + 0.5 * (double)s.n_seqs);       // sequences are not whole segments
-        const double folded = 0.2 * (double)(s.longest / k);        // a segment takes in the ones before it
-        const double time = scan_time(ctas, (double)k, walk) + scan_time(ctas, (double)k, first) + 4.0 + folded;
+        const double per_seq = std::ceil(longest / k), pieces = s.packed ? s.num_chunks / (double)k + 0.5 * s.n_seqs : s.n_seqs * per_seq, ctas = pieces * tiles;
+        const double folded = fit.folded * per_seq * std::max(1.0, ctas / (2.0 * SMS));
+        const double time = scan_time(ctas, (double)k, work, walk, fit) + scan_time(ctas, (double)k, work, first, fit) + 2.0 + folded;
         if (time < 0.95 * best) {
             best = time;
             seg = k;
@@ -147,7 +155,7 @@ ScanOutputs scan_forward(const ScanInputs& in, bool want_final, bool keep) {
     }
     cula_kda_selective_scan_args a = scan_args(in, s);
     a.y = ptr(o.y); a.hT = fptr(o.hT); a.states = fptr(o.states); a.y_pre = fptr(o.y_pre);
-    a.seg_chunks = (int)plan_segments(s, 1.0);
+    a.seg_chunks = (int)plan_segments(s, false);
     Tensor seg;
     if (a.seg_chunks) {
         const int64_t n = segment_slots(s, in, a.seg_chunks);
@@ -212,7 +220,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         a.states = fptr(v[8]); a.y_pre = fptr(v[9]); a.dy = ptr(dy); a.dhT = fptr(dhT);
         a.dx = ptr(dx); a.ddt = ptr(ddt); a.dz = ptr(dz); a.dBm = ptr(dB); a.dCm = ptr(dC);
         a.dA = fptr(dA); a.dskip = fptr(dskip); a.dbias = fptr(dbias); a.dh0 = fptr(dh0);
-        a.seg_chunks = (int)plan_segments(s, 0.5);
+        a.seg_chunks = (int)plan_segments(s, true);
         const int64_t n_seg = segment_slots(s, in, a.seg_chunks);
         const int64_t items = a.seg_chunks ? n_seg : s.n_seqs;
         a.cta_rows = (int)std::max<int64_t>(1, std::min(items, 8 * SMS / s.tiles));

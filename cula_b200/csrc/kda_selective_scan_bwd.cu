@@ -12,25 +12,9 @@
 namespace kda {
 
 constexpr int SEL_BWD_THREADS = 2 * SEL_THREADS;
-constexpr int SEL_SCAN_REGS = 192, SEL_SERVE_REGS = 64;             // of a thread of either kind; the block is launched with their mean
+constexpr int SEL_SCAN_REGS = 184, SEL_SERVE_REGS = 72;             // of a thread of either kind; the block is launched with their mean
 
 __device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(SEL_BWD_THREADS) : "memory"); }
-
-// Sums over the channels of a warp for gradients in 16 bits (dB, dC) go over neighbouring lanes by matrix instructions that multiply with
-// ones: 2 of them and 4 other instructions per token instead of 28, 7 of which are exchanges through shared memory's data path, which
-// bounds this kernel. The instruction drops all but 10 bits behind the leading one of a thread's value (two channels' sum; further sums are
-// fp32): independent errors of at most 2^-10 of a term, against the 2^-8 of the result's own rounding. Their mean, 2^-11 (1 - 1/2) / ln 2 for
-// evenly spread exponents, is put back at the end. 16 lanes over states leave too few neighbours over channels.
-template <int SL, typename T>
-constexpr bool sel_tensor_sums() { return sizeof(T) == 2 && SL <= 8; }
-constexpr float SEL_DROPPED = 1.f + 0.7213475f / 2048.f;
-// c += what (a0, a2) are over four neighbouring lanes, in the columns that b0, b1 mark; likewise (a1, a3) eight rows below
-__device__ __forceinline__ void sel_sum4(float (&c)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)), "r"(__float_as_uint(b0)),
-          "r"(__float_as_uint(b1)));
-}
 
 template <int SL, typename T>
 struct SelBwdSmem {
@@ -277,11 +261,6 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
         }
     }
 
-    constexpr bool TENSOR = !STATE_ONLY && sel_tensor_sums<SL, T>();
-    float ones[8];                                                   // columns of the sums on tensor cores
-#pragma unroll
-    for (int k = 0; k < 8; ++k) ones[k] = (lane >> 2) == k ? 1.f : 0.f;
-
     for (long long i = row; i < items; i += a.cta_rows) {
         SelItem it;
         if (!sel_item(a, i, it) || (STATE_ONLY && it.seg == 0)) continue;        // nothing comes before a first segment
@@ -368,7 +347,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                         }
                     }
                     constexpr int TB = SL > 4 ? SL / 4 : 2;          // tokens whose sums over states are added up together
-                    float v[4 * TB], bc[4];
+                    float v[4 * TB];
                     // the next token's rows are asked for before this one's sums are stored: no load waits behind a store
                     float4 dx_n = sm.dx[buf][tb + KEEP - 1][pair], b_n = sm.b[buf][tb + KEEP - 1][s], c_n = sm.c[buf][tb + KEEP - 1][s];
                     float2 dy_n = sm.dy[buf][tb + KEEP - 1][pair];
@@ -413,39 +392,20 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                             else if constexpr (LEFT == 2) *reinterpret_cast<float2*>(to) = make_float2(r[0], r[1]);
                             else *to = r[0];
                         }
-                        if constexpr (TENSOR) {
-                            // columns of the token of two: states n0..n0+3; rows: dB and (below) dC of the lanes' quads
-                            const int w = 4 * (u & 1);
-                            if (u & 1) bc[0] = bc[1] = bc[2] = bc[3] = 0.f;
-                            sel_sum4(bc, dB0.x, dC0.x, dB0.y, dC0.y, ones[w], ones[w + 1]);
-                            sel_sum4(bc, dB1.x, dC1.x, dB1.y, dC1.y, ones[w + 2], ones[w + 3]);
-                            if (!(u & 1)) {
-                                constexpr int HI = CL / 4, LEFT = 4 / HI;        // quads of lanes over channels, values that each lane is left with
-                                sel_reduce<4, HI>(bc, lane, 4);
-                                float* to = sm.bc[buf][warp][tb + u + ((lane >> 1) & 1)] + n0 + 2 * (lane & 1);
-#pragma unroll
-                                for (int k = 0; k < LEFT; k += LEFT > 1 ? 2 : 1) {
-                                    const int id = (cl >> 2) * LEFT + k;
-                                    if constexpr (LEFT > 1) *reinterpret_cast<float2*>(to + (id >> 1) * SP) = make_float2(bc[k], bc[k + 1]);
-                                    else to[(id >> 1) * SP + (id & 1)] = bc[k];
-                                }
+                        float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
+                        sel_reduce<8, CL>(r, lane, 1);
+                        if constexpr (CL >= 8) {
+                            constexpr int REP = CL / 8;          // lanes left with the same value
+                            if (REP == 1 || cl % REP == 0) {
+                                const int id = cl / REP;
+                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
                             }
                         } else {
-                            float r[8] = {dB0.x, dB0.y, dB1.x, dB1.y, dC0.x, dC0.y, dC1.x, dC1.y};
-                            sel_reduce<8, CL>(r, lane, 1);
-                            if constexpr (CL >= 8) {
-                                constexpr int REP = CL / 8;          // lanes left with the same value
-                                if (REP == 1 || cl % REP == 0) {
-                                    const int id = cl / REP;
-                                    sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
-                                }
-                            } else {
-                                constexpr int LEFT = 8 / CL;
+                            constexpr int LEFT = 8 / CL;
 #pragma unroll
-                                for (int k = 0; k < LEFT; ++k) {
-                                    const int id = cl * LEFT + k;
-                                    sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
-                                }
+                            for (int k = 0; k < LEFT; ++k) {
+                                const int id = cl * LEFT + k;
+                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
                             }
                         }
                     }
@@ -482,8 +442,7 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
 // ---- the shares added up: dB and dC (four threads per token row, group and four states, one after the other's part of the shares), then dA,
 //      dskip, dbias (one thread per value) ----
 template <typename T>
-__global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks,
-                                                                    const float scale) {
+__global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelScanArgs a, const int tiles_per_group, const int SP, const unsigned bc_blocks) {
     __shared__ float4 part[3][64];
     pdl_launch_dependents();
     pdl_wait();
@@ -508,7 +467,7 @@ __global__ void __launch_bounds__(256) kda_selective_scan_sum_kernel(const SelSc
             sum.x += r.x; sum.y += r.y; sum.z += r.z; sum.w += r.w;
         }
         T* to = static_cast<T*>(isC ? a.dCm : a.dBm) + rg * a.S;
-        const float f[4] = {sum.x * scale, sum.y * scale, sum.z * scale, sum.w * scale};
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if (n + k < a.S) {
@@ -561,8 +520,7 @@ static int launch_sel_bwd(const SelScanArgs& a, cudaStream_t stream) {
         return (int)e;
     const long long bc_blocks = (a.rows * a.G * (G::SP / 2) + 63) / 64, rest = ((long long)a.D * (G::SP + 2) + 255) / 256;
     if (bc_blocks + rest > 0x7fffffffLL) return -1;
-    return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks,
-                             sel_tensor_sums<SL, T>() ? SEL_DROPPED : 1.f);
+    return (int)launch_early(kda_selective_scan_sum_kernel<T>, dim3((unsigned)(bc_blocks + rest)), 256, 0, stream, a, tpg, G::SP, (unsigned)bc_blocks);
 }
 
 }  // namespace kda
