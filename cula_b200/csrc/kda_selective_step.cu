@@ -291,7 +291,7 @@ extern "C" int kda_launch_selective_step(const kda::SelStepArgs* a, cudaStream_t
 extern "C" int kda_launch_conv_step(const kda::ConvStepArgs* a, cudaStream_t stream) {
     using namespace kda;
     if (a->rows == 0) return 0;
-    const StepGrid g = step_grid(a->rows, a->D / 2, 12);
+    const StepGrid g = step_grid(a->rows, a->D / 2, 16);
     void (*kernel)(const ConvStepArgs, const int, const int) = a->W == 1 ? kda_conv_step_kernel<1> : a->W == 2 ? kda_conv_step_kernel<2>
                                                              : a->W == 3 ? kda_conv_step_kernel<3> : kda_conv_step_kernel<4>;
     return (int)launch_early(kernel, dim3((unsigned)(g.tiles * g.row_step)), g.threads, 0, stream, *a, g.tiles, g.row_step);
