@@ -493,7 +493,8 @@ int scan_args_error(const kda::SelScanArgs* a) {
     const bool packed = a->cu_seqlens != nullptr;
     if (packed != (a->chunk_indices != nullptr) || packed != (a->chunk_offsets != nullptr) || packed != (a->seq_order != nullptr)) return CULA_KDA_EINVAL;
     if (packed && (a->total_tokens < 0 || a->total_tokens > a->rows)) return CULA_KDA_EINVAL;
-    if (!packed && a->T < 0) return CULA_KDA_EINVAL;
+    if (!packed && (a->T < 0 || a->rows != (long long)a->n_seqs * a->T || a->num_chunks != (long long)a->n_seqs * ((a->T + kda::BT - 1) / kda::BT)))
+        return CULA_KDA_EINVAL;
     if (a->seg_chunks && (!a->seg_state || !a->seg_dt)) return CULA_KDA_EINVAL;
     const int per = a->fp32 ? 4 : 8;
     if (misaligned(a->x) || misaligned(a->dt) || misaligned(a->z) || a->x_row % per || a->dt_row % per || a->x_seq % per || a->dt_seq % per ||

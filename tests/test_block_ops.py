@@ -135,12 +135,9 @@ def test_norm_with_one_gradient_only_and_views():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("R,D,dtype,res", NORMS)
-@pytest.mark.parametrize("group", [None, 32, 128, 256])
+@pytest.mark.parametrize("R,D,dtype,res,group", [(*n, g) for n in NORMS for g in (None, 32, 128, 256) if g is None or n[1] % g == 0])
 def test_norm_in_8_bits(R, D, dtype, res, group):
     from cula_b200.kda import add_rms_norm_fp8
-    if group and D % group:
-        pytest.skip("columns are not whole groups")
     x, w, r = norm_inputs(R, D, dtype, res, seed=2)
     y_ref, v_ref = add_rms_norm_ref(x.double(), w.double(), None if r is None else r.double(), eps=1e-5, stream=None if r is None else r.dtype)
     q_ref, s_ref = quantize_e4m3_ref(y_ref, group)
@@ -174,7 +171,64 @@ def test_norm_in_8_bits_of_zeros_infinities_and_nan(D):
         assert q[3].isfinite().all() and q[4].isfinite().all() and s[3:].isfinite().all()
 
 
+@pytest.mark.gpu
+def test_norm_past_32_bits_and_in_a_cuda_graph_on_another_stream():
+    from cula_b200.kda import add_rms_norm, add_rms_norm_fp8
+    D = 8192
+    R = 2 ** 31 // D + 3
+    x = torch.empty(R, D, device="cuda", dtype=torch.bfloat16).fill_(1.0)
+    x[-2:] = torch.randn(2, D, device="cuda").bfloat16()
+    w = torch.ones(D, device="cuda", requires_grad=True)
+    y, _ = add_rms_norm(x, w, x)
+    y2, _ = add_rms_norm(x[-2:], w, x[-2:])
+    assert torch.equal(y[-2:], y2)
+    q, s, _ = add_rms_norm_fp8(x, w, x, group_size=128)
+    q2, s2, _ = add_rms_norm_fp8(x[-2:], w, x[-2:], group_size=128)
+    assert torch.equal(q[-2:].float(), q2.float()) and torch.equal(s[-2:], s2)
+    dy = torch.zeros_like(y)
+    dy[-2:] = 1.0
+    g, = torch.autograd.grad(y, w, dy)
+    g2, = torch.autograd.grad(y2, w, dy[-2:])
+    assert err_ratio(g2.double().cpu(), g.double().cpu()) < FP32
+    del x, y, q, s, dy
+    torch.cuda.empty_cache()
+    x, r = torch.randn(70, 264, device="cuda").bfloat16().requires_grad_(True), torch.randn(70, 264, device="cuda", requires_grad=True)
+    w = torch.rand(264, device="cuda", requires_grad=True)
+
+    def step():
+        y, v = add_rms_norm(x, w, r)
+        return [y.detach(), v.detach(), *torch.autograd.grad([y, v], [x, w, r], [torch.ones_like(y), torch.ones_like(v)])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = [t.clone() for t in step()]
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for t, u in zip(static, eager):
+        assert torch.equal(t, u)
+
+
 # ------------------------------------------------ short convolution, single tokens ------------------------------------------------
+@pytest.mark.gpu
+def test_conv_step_in_a_pool_past_32_bits():
+    from cula_b200.kda import short_conv_update
+    D = 12288
+    slots = 2 ** 31 // (D * 4) + 3
+    pool = torch.empty(slots, D, 4, device="cuda")
+    small = torch.randn(2, D, 4, device="cuda")
+    pool[0], pool[slots - 1] = small[0], small[1]
+    x, w = torch.randn(2, D, device="cuda").bfloat16(), torch.randn(D, 4, device="cuda")
+    y = short_conv_update(x, w, pool, torch.tensor([0, slots - 1], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, short_conv_update(x, w, small)) and torch.equal(pool[0], small[0]) and torch.equal(pool[slots - 1], small[1])
+    del pool
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("N,D,W,bias,act,indexed", [(1, 8, 4, True, "silu", False), (3, 264, 3, False, "silu", True), (33, 1032, 4, True, None, True),
                                                     (5, 520, 2, True, "swish", True), (2, 16, 1, False, "silu", False), (700, 512, 4, True, "silu", True)])

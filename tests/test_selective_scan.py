@@ -121,6 +121,22 @@ def test_refusals():
             selective_scan_update(**s)
 
 
+def test_c_entries_refuse_what_they_cannot_do():
+    """No null structure, no sizes that contradict each other: an error code before anything is launched."""
+    import ctypes
+
+    from cula_b200 import _native
+    lib = _native.lib()
+    for name in ("selective_scan_fwd", "selective_scan_bwd", "selective_step", "conv_step", "add_rms_norm_fwd", "add_rms_norm_bwd"):
+        call = getattr(lib, "cula_kda_" + name)
+        assert call(None, None) == -1
+        zeros = ctypes.create_string_buffer(1024)                   # every size zero, every pointer null
+        assert call(ctypes.byref(zeros), None) in (0, -1)
+    assert lib.cula_kda_selective_scan_tiles(64, 1, 65) == -1 and lib.cula_kda_selective_scan_tiles(200, 1, 16) == 4
+    assert lib.cula_kda_selective_scan_state_floats(200, 1, 16) == 4 * 1024 and lib.cula_kda_selective_scan_state_floats(0, 1, 16) == -1
+    assert lib.cula_kda_add_rms_norm_shares(128, 0) == 0
+
+
 # ------------------------------------------------------------------ GPU ------------------------------------------------------------------
 def check_all(a, cu=None, want_final=True, seed=9, names=None):
     """Outputs and every gradient of a call against the oracle's."""
@@ -344,7 +360,75 @@ def test_forward_and_backward_in_a_cuda_graph_on_another_stream():
         assert torch.equal(t, u)
 
 
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    """More than 2^31 elements per tensor: the last tokens, forward and backward, against a call on them alone."""
+    from cula_b200.kda import selective_scan
+    D, S, tail = 1024, 16, 300
+    T = 2 ** 31 // D + 128 + tail
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(1, T, D, device="cuda", dtype=torch.bfloat16).fill_(0.5)
+    x[:, -tail - 200:] = torch.randn(1, tail + 200, D, device="cuda", generator=gen).bfloat16()
+    dt = torch.full((1, 1, D), -1.0, device="cuda", dtype=torch.bfloat16).expand(1, T, D)
+    bc = torch.randn(1, 1, S, device="cuda", generator=gen).bfloat16().expand(1, T, S)
+    A = -torch.rand(D, S, device="cuda", generator=gen) - 0.05
+    x.requires_grad_(True)
+    y, fin = selective_scan(x, dt, A, bc, bc, dt_softplus=True, output_final_state=True)
+    with torch.no_grad():
+        _, h = selective_scan(x[:, :-tail], dt[:, :-tail], A, bc[:, :-tail], bc[:, :-tail], dt_softplus=True, output_final_state=True)
+    part = x.detach()[:, -tail:].clone().requires_grad_(True)
+    y2, fin2 = selective_scan(part, dt[:, -tail:], A, bc[:, -tail:], bc[:, -tail:], dt_softplus=True, initial_state=h, output_final_state=True)
+    assert err_ratio(y2.detach().double().cpu(), y.detach()[:, -tail:].double().cpu()) < tol(torch.bfloat16, tail)
+    assert err_ratio(fin2.detach().double().cpu(), fin.detach().double().cpu()) < 2 * tol(torch.float32, tail)
+    dy2 = torch.randn(y2.shape, device="cuda", generator=gen).bfloat16()
+    dy = torch.zeros_like(y)
+    dy[:, -tail:] = dy2
+    del y2, h
+    g, = torch.autograd.grad(y, x, dy)
+    g2, = torch.autograd.grad(selective_scan(part, dt[:, -tail:], A, bc[:, -tail:], bc[:, -tail:], dt_softplus=True)[0], part, dy2)
+    assert err_ratio(g2.double().cpu(), g[:, -tail:].double().cpu()) < 2 * tol(torch.bfloat16, tail)
+    del x, y, dy, g
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------ one token ------------------------------------------------------------------
+@pytest.mark.gpu
+def test_step_in_a_pool_past_32_bits():
+    from cula_b200.kda import selective_scan_update
+    D, S = 4096, 64
+    slots = 2 ** 31 // (D * S) + 3
+    pool = torch.empty(slots, D, S, device="cuda")
+    small = torch.randn(2, D, S, device="cuda")
+    pool[0], pool[slots - 1] = small[0], small[1]
+    a = on_gpu({k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in make(2, 1, D, S, seed=3).items()})
+    del a["initial_state"]
+    y = selective_scan_update(**a, state=pool, state_indices=torch.tensor([0, slots - 1], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, selective_scan_update(**a, state=small)) and torch.equal(pool[0], small[0]) and torch.equal(pool[slots - 1], small[1])
+    del pool
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_steps_in_a_cuda_graph():
+    from cula_b200.kda import selective_scan_update
+    a = on_gpu({k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in make(40, 1, 256, 16, seed=5).items()})
+    del a["initial_state"]
+    start = torch.randn(50, 256, 16, device="cuda")
+    idx = torch.randperm(50, device="cuda")[:40].to(torch.int32)
+    pool, eager = start.clone(), start.clone()
+    y0 = selective_scan_update(**a, state=eager, state_indices=idx)
+    y1 = selective_scan_update(**a, state=eager, state_indices=idx)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = selective_scan_update(**a, state=pool, state_indices=idx)
+    pool.copy_(start)
+    for ref in (y0, y1):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref)
+    assert torch.equal(pool, eager)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("N,D,S,G,dtype,gate,indexed", [(1, 8, 1, 1, "bf16", True, False), (3, 40, 16, 1, "fp32", True, True), (5, 264, 12, 1, "bf16", False, True),
                                                         (2, 48, 5, 3, "fp32", True, False), (4, 64, 33, 2, "bf16", True, True), (2, 16, 64, 1, "fp32", True, True),
