@@ -7,6 +7,15 @@
 // those that the forward pass kept, and stay in registers together with the a_t until the way back has used them. Sums over states go over
 // the lanes of a channel, sums over channels over the lanes of a state and the warps; the tiles' shares of dB and dC and the CTAs' shares
 // of dA, dskip and dbias are added up by a second kernel in a fixed order, so that every gradient is the same from run to run.
+//
+// Four warps scan, with the 136 registers that eight tokens' states and factors take, and four serve them as in the forward pass: rows two
+// tiles ahead, operands of the next tile, gradients of the tile before. Per element one exponential, eleven multiply-adds (packed in
+// pairs) and two sums over lanes, which go as half of the values per step. At 4 x 2048 x 4096 x 16 in bf16 with a gate (473 MB): 73 us of
+// traffic, 115 (145) us of exponentials, 184 us of multiply-adds at their rate. Measured: 1040 us with every thread doing everything, 566
+// so (lone CTAs 345). Nothing is saturated: issue slots 58 %, of which packed multiply-adds take two each, shared memory's data path 53 %
+// of the launch; 22 % of the warps that would fit are resident, since registers and shared memory hold two CTAs per SM. Tried: sums over
+// channels by tensor-core products with ones (590: fewer exchanges, no less time), packed pairs over channels in place of states (689: B
+// and C twice in shared memory), eight scanning warps and four serving ones in one CTA per SM (617), other register splits (176 + 80: 592).
 #include "selective_scan.cuh"
 
 namespace kda {

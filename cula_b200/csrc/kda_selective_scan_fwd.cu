@@ -2,6 +2,12 @@
 // tokens at a time. Four warps scan: every (token, channel, state) costs one exponential and four multiply-adds (packed in pairs) on
 // states that stay in registers. Four others serve them: they fetch the rows of the tiles ahead, make the steps and their products with x,
 // once per token and channel, for the next tile, and turn the sums of the tile before into outputs. One barrier per tile.
+//
+// What it cannot do without at 4 x 2048 tokens x 4096 channels x 16 states in bf16 with a gate (268 MB): 42 us of HBM traffic, 115 us of
+// exponentials (16 per clock and SM), 145 with those of softplus and silu. Measured: 524 us with every thread staging, scanning and writing
+// in turn (B and C rows waited for in registers, 16-byte loads of 32 lanes to 32 lines for the kept states), 226 us so; 239 with the
+// states kept for a backward pass. The unit of the exponentials is 64 % busy: 256 CTAs leave 40 of 148 SMs with one CTA in place of two
+// (86 %), and of a pair's time it is busy for three quarters; the data path of shared memory is half busy beside it.
 #include "selective_scan.cuh"
 
 namespace kda {
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
     for (int k = 0; k < n_tiles; ++k) {
         const int buf = k & 1;
         // The sums over states come after the tile's last token: everything before is independent of their exchanges, and no shared store
-        // stands between its loads (token by token a lone warp took 490 cycles per token, now 190).
+        // stands between its loads. A warp alone on its scheduler takes 125 cycles per token, two of them 103 each; 65 are exponentials.
         float v[2 * LC];
 #pragma unroll
         for (int u = 0; u < LC; ++u) {

@@ -60,8 +60,9 @@ __device__ __forceinline__ int step_slot(const int* indices, int row, int pool, 
 // SL lanes (four states each) share a channel, NI channels a lane: channel c of lane (g, s) is the warp's c (32 / SL) + g. What concerns a
 // channel as a whole (step, gate, output) is done by one lane, its owner, and handed to the others. The states of the next two rows are
 // on their way to shared memory, each thread's to a place of its own, while a row is worked on; everything else is asked for one row ahead.
-// Measured at 256 rows x 4096 channels x 16 states in bf16 (144 MB): 65 us with a block per row and tile, 29 with rows walked and one
-// ahead in registers.
+// Bound by memory: 256 rows x 4096 channels x 16 states in bf16 (143 MB, 22 us at the copy rate) take 65 us with a block per row and tile
+// and 28.8 so (5.0 TB/s, launch and ramp included; 512 rows 5.3). One row ahead in registers: 29.3, and 46 in the place of 28 where 64
+// states leave none. A ring of 2 or 4 rows: 33, 35.
 constexpr int STEP_RING = 3;
 
 template <int SL, typename T>
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_selective_step_kernel(const 
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// two neighbouring channels per thread
+// two neighbouring channels per thread; 256 rows x 12288 channels x 4 (113 MB, 17.6 us at the copy rate): 20.1 us
 template <int W>
 __global__ void __launch_bounds__(STEP_THREADS) kda_conv_step_kernel(const ConvStepArgs a, const int tiles, const int row_step) {
     const int d0 = 2 * ((blockIdx.x % tiles) * blockDim.x + threadIdx.x);
