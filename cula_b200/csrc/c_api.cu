@@ -496,6 +496,12 @@ int scan_args_error(const kda::SelScanArgs* a) {
     if (!packed && (a->T < 0 || a->rows != (long long)a->n_seqs * a->T || a->num_chunks != (long long)a->n_seqs * ((a->T + kda::BT - 1) / kda::BT)))
         return CULA_KDA_EINVAL;
     if (a->seg_chunks && (!a->seg_state || !a->seg_dt)) return CULA_KDA_EINVAL;
+    for (const long long row : {a->x_row, a->dt_row, a->z ? a->z_row : 0, a->b_row, a->c_row})
+        if (row < 0 || row > 0x7fffffffLL) return CULA_KDA_EINVAL;
+    const uintptr_t quad = a->fp32 ? 15 : 7;
+    if (a->vec_bc && ((a->S % 4 && a->G > 1) || ((reinterpret_cast<uintptr_t>(a->Bm) | reinterpret_cast<uintptr_t>(a->Cm)) & quad) || a->b_row % 4 ||
+                      a->c_row % 4 || a->b_seq % 4 || a->c_seq % 4))
+        return CULA_KDA_EALIGN;
     const int per = a->fp32 ? 4 : 8;
     if (misaligned(a->x) || misaligned(a->dt) || misaligned(a->z) || a->x_row % per || a->dt_row % per || a->x_seq % per || a->dt_seq % per ||
         (a->z && (a->z_row % per || a->z_seq % per)) || misaligned(a->states) || misaligned(a->seg_state) || misaligned(a->seg_dt) || misaligned(a->y_pre))
@@ -539,7 +545,10 @@ extern "C" int cula_kda_selective_step(const cula_kda_selective_step_args* a, vo
     if (!a->x || !a->dt || !a->Bm || !a->Cm || !a->A || !a->state || !a->y || !a->status || a->D <= 0 || a->G <= 0 || a->D % a->G || a->S <= 0 || a->S > 64)
         return CULA_KDA_EINVAL;
     if (!a->indices && a->pool < a->rows) return CULA_KDA_EINVAL;
-    if (a->vec && (a->S % 4 || misaligned(a->state) || misaligned(a->A))) return CULA_KDA_EALIGN;
+    const uintptr_t quad = a->fp32 ? 15 : 7;
+    if (a->vec && (a->S % 4 || misaligned(a->state) || misaligned(a->A) || a->b_row % 4 || a->c_row % 4 ||
+                   ((reinterpret_cast<uintptr_t>(a->Bm) | reinterpret_cast<uintptr_t>(a->Cm)) & quad)))
+        return CULA_KDA_EALIGN;
     return checked(kda_launch_selective_step(a, static_cast<cudaStream_t>(stream)));
 }
 

@@ -313,7 +313,7 @@ int cula_kda_rms_norm_gated_bwd(const void* d_x, const void* d_g, const float* d
  *     step_t = softplus(dt_t + dt_bias) (or without softplus),   h_t = exp(step_t A) h_{t-1} + step_t x_t B_t
  *     y_t = (sum_n C_t[n] h_t[n] + skip x_t) silu(z_t)
  * Rows of x, dt, z, B and C may be strided (row: elements from a token to the next, seq: from a sequence of a fixed-length batch to the
- * next); their innermost dimensions are contiguous, rows of x, dt and z are 16-byte aligned, D / G is a multiple of 8, S <= 64. Everything
+ * next; row strides fit 31 bits); their innermost dimensions are contiguous, rows of x, dt and z are 16-byte aligned, D / G is a multiple of 8, S <= 64. Everything
  * else is contiguous. A sequence is walked in one piece, or (seg_chunks) in segments of that many 64-token chunks side by side, for which a
  * launch before finds what each adds to the state.
  * SP below is the smallest of 8, 16, 32 and 64 that holds S.

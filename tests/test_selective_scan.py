@@ -292,6 +292,23 @@ def test_gradients_are_the_same_from_run_to_run_and_agree_with_differences():
 
 
 @pytest.mark.gpu
+def test_parameters_in_16_bits_and_one_tensor_in_several_places():
+    """bf16 parameters get bf16 gradients; x passed as dt and z too gets the sum of theirs."""
+    from cula_b200.kda import selective_scan
+    a = make(2, 40, 24, 6, h0=0, seed=8)
+    a = {**a, "dt": None, "z": None, **{k: a[k].bfloat16() for k in ("A", "D", "dt_bias")}}
+    r, d = in64(a, True), on_gpu(a, True)
+    y_ref, _ = selective_scan_ref(**{**r, "dt": r["x"], "z": r["x"]})
+    y, _ = selective_scan(**{**d, "dt": d["x"], "z": d["x"]})
+    names = ["x", "A", "B", "C", "D", "dt_bias"]
+    got, ref = torch.autograd.grad(y.float().sum(), [d[k] for k in names]), torch.autograd.grad(y_ref.sum(), [r[k] for k in names])
+    assert err_ratio(y_ref.detach(), y.detach().double().cpu()) < tol(torch.bfloat16, 40)
+    for k, g, h in zip(names, got, ref):
+        # three gradients of x are rounded one by one and their sum twice more
+        assert g.dtype == torch.bfloat16 and err_ratio(h, g.double().cpu()) < (5 if k == "x" else 1) * tol(torch.bfloat16, 40), k
+
+
+@pytest.mark.gpu
 def test_only_one_result_is_differentiated():
     from cula_b200.kda import selective_scan
     a = make(1, 30, 16, 4, 1, torch.float32, h0=1)
