@@ -2,6 +2,9 @@
 #include <algorithm>
 #include <climits>
 
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+
 #include "host_common.h"
 
 namespace cula_host {
@@ -55,6 +58,21 @@ Tensor rows_of(const Tensor& t, int64_t inner_dims) {
     return t.is_contiguous() ? t.clone() : t.contiguous();
 }
 long long stride_of(const Tensor& t, int64_t d) { return t.size(d) == 1 ? 0 : t.stride(d); }
+
+// A backward pass that is captured into a graph while an eager graph of the same leaves lives on the default stream: their accumulators belong
+// to that stream, the engine would wait on it across the capture, and that ends the process. Said here, before it happens. (Accumulators
+// of other streams can be waited on.)
+void refuse_accumulators_of_the_default_stream(const Tensor& like) {
+    if (at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const c10::Stream outside = c10::cuda::getDefaultCUDAStream(like.device().index()).unwrap();
+    for (const auto& edge : node->next_edges())
+        if (edge.function && dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()))
+            if (const auto stream = edge.function->stream(); stream.has_value() && *stream == outside)
+                throw std::runtime_error("a backward pass cannot be captured while an earlier graph of the same leaves lives: its outputs hold their "
+                                         "gradient accumulators, which belong to the default stream; let go of them first");
+}
 
 // ------------------------------------------------ selective scan ------------------------------------------------
 int64_t padded_states(int64_t S) { return S <= 8 ? 8 : S <= 16 ? 16 : S <= 32 ? 32 : 64; }
@@ -190,6 +208,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         const Tensor dhT = grads.size() > 1 && grads[1].defined() ? contiguous_f32(grads[1]) : Tensor();
         if (!grads[0].defined() && !dhT.defined()) return out;
         auto v = ctx->get_saved_variables();
+        refuse_accumulators_of_the_default_stream(v[0]);
         ScanInputs in{v[0], v[1], v[2], v[3], v[4], opt_of(v[5]), opt_of(v[6]), opt_of(v[7]), OptTensor(), ctx->saved_data["softplus"].toBool(), std::nullopt};
         if (auto it = ctx->saved_data.find("tab"); it != ctx->saved_data.end()) {
             auto t = it->second.toTensorVector();
@@ -451,6 +470,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         if (!grads[0].defined() && (!with_r || !grads[1].defined())) return variable_list(4);
         auto s = ctx->get_saved_variables();
         const Tensor &v = s[0], &w = s[1], &rstd = s[2];
+        refuse_accumulators_of_the_default_stream(v);
         const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();
         const int64_t res = ctx->saved_data["res"].toInt(), D = v.size(-1), R = v.numel() / D;
         c10::cuda::CUDAGuard guard(v.device());

@@ -213,6 +213,38 @@ def test_norm_past_32_bits_and_in_a_cuda_graph_on_another_stream():
         assert torch.equal(t, u)
 
 
+@pytest.mark.gpu
+def test_capture_beside_a_living_eager_graph_is_refused():
+    """The engine would end the process; the operators' backward passes say what is wrong instead, and the capture works afterwards."""
+    from cula_b200.kda import add_rms_norm, selective_scan
+    x = torch.randn(1, 40, 64, device="cuda").bfloat16().requires_grad_(True)
+    w, A = torch.rand(64, device="cuda", requires_grad=True), -torch.rand(64, 8, device="cuda") - 0.1
+    bc = torch.randn(1, 40, 8, device="cuda").bfloat16()
+    for call in (lambda: add_rms_norm(x, w)[0], lambda: selective_scan(x, x, A, bc, bc, dt_softplus=True)[0]):
+        def step(call=call):
+            y = call()
+            return torch.autograd.grad(y, x, torch.ones_like(y))[0]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = step().clone()
+        side.synchronize()
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="earlier graph of the same leaves"):
+            with torch.cuda.graph(graph):
+                step()
+        torch.cuda.synchronize()
+        del alive, graph
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            static = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(static, eager)
+
+
 # ------------------------------------------------ short convolution, single tokens ------------------------------------------------
 @pytest.mark.gpu
 def test_conv_step_in_a_pool_past_32_bits():
