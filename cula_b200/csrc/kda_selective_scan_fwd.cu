@@ -5,9 +5,10 @@
 //
 // What it cannot do without at 4 x 2048 tokens x 4096 channels x 16 states in bf16 with a gate (268 MB): 42 us of HBM traffic, 115 us of
 // exponentials (16 per clock and SM), 145 with those of softplus and silu. Measured: 524 us with every thread staging, scanning and writing
-// in turn (B and C rows waited for in registers, 16-byte loads of 32 lanes to 32 lines for the kept states), 226 us so; 239 with the
-// states kept for a backward pass. The unit of the exponentials is 64 % busy: 256 CTAs leave 40 of 148 SMs with one CTA in place of two
-// (86 %), and of a pair's time it is busy for three quarters; the data path of shared memory is half busy beside it.
+// in turn (B and C rows waited for in registers, 16-byte loads of 32 lanes to 32 lines for the kept states), 219 us so; 234 with the
+// states kept for a backward pass. The unit of the exponentials is 66 % busy: 256 CTAs leave 40 of 148 SMs with one CTA in place of two
+// (86 %), and of a pair's time it is busy for three quarters; the data path of shared memory is half busy beside it. An eighth or a quarter
+// of the exponentials as polynomials on the multiply-add units made it 6 and 9 us slower.
 #include "selective_scan.cuh"
 
 namespace kda {
@@ -24,7 +25,6 @@ struct SelFwdSmem {
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float4 b[2][G::LC][G::SL], c[2][G::LC][G::SL];
     float2 y[2][G::LC][G::CH / 2 + 2];                               // rows shifted against each other: no bank conflicts of the writers
-    float2 par[2][4][G::VECS];                                       // dt_bias, skip: [which][pair of a piece][piece]
     T raw_b[SEL_AHEAD][G::UNITS][4], raw_c[SEL_AHEAD][G::UNITS][4];                  // B and C rows as they are
     uint4 raw[SEL_AHEAD][3][Q][G::ITEMS];                                    // x, dt, z rows as they are: [stage][which][piece][thread]
 };
@@ -83,35 +83,33 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
             }
             sel_commit();
         };
-        for (int i = tid; i < CH; i += SEL_THREADS) {
-            const bool in = d0 + i < d_end;
-            (&sm.par[0][i / 2 % 4][i / 8].x)[i & 1] = in && a.dt_bias ? a.dt_bias[d0 + i] : 0.f;
-            (&sm.par[1][i / 2 % 4][i / 8].x)[i & 1] = in && a.skip ? a.skip[d0 + i] : 0.f;
-        }
-        asm volatile("bar.sync 2, %0;" :: "n"(SEL_THREADS) : "memory");
-        auto param = [&](int which, float2 (&v)[4]) {
+        float2 bias[4], skip[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = sm.par[which][e][tid % G::VECS];
-        };
+        for (int e = 0; e < 4; ++e) {
+            bias[e] = item && a.dt_bias ? make_float2(a.dt_bias[dv + 2 * e], a.dt_bias[dv + 2 * e + 1]) : make_float2(0.f, 0.f);
+            skip[e] = !STATE_ONLY && item && a.skip ? make_float2(a.skip[dv + 2 * e], a.skip[dv + 2 * e + 1]) : make_float2(0.f, 0.f);
+        }
         auto stage = [&](int k) {                                        // tile k, arrived, as the scan takes it; zeros past the end change no state
             const int buf = k & 1, slot = k % SEL_AHEAD;
             if (tid < G::ITEMS) {
-                const bool live = item && it.t0 + k * LC + tt < it.t1;
                 const uint4(*from)[Q][G::ITEMS] = sm.raw[slot];
-                float2 x[4], d[4], b[4];
+                float2 x[4], d[4];
                 V::unpack(&from[0][0][tid], G::ITEMS, x);
                 V::unpack(&from[1][0][tid], G::ITEMS, d);
-                param(0, b);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d[e] = add2(d[e], b[e]);
+                for (int e = 0; e < 4; ++e) d[e] = add2(d[e], bias[e]);
                 if (a.softplus) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) d[e] = sel_softplus2(d[e]);
                 }
+                if (!(item && it.t0 + k * LC + tt < it.t1)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[e] = x[e] = make_float2(0.f, 0.f);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float2 p = mul2(d[e], x[e]);
-                    sm.dx[buf][tt][e * G::VECS + tid % G::VECS] = live ? make_float4(d[e].x, d[e].y, p.x, p.y) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    sm.dx[buf][tt][e * G::VECS + tid % G::VECS] = make_float4(d[e].x, d[e].y, p.x, p.y);
                 }
             }
 #pragma unroll
@@ -133,9 +131,8 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
             const int t = it.t0 + k * LC + tt;
             if (item && t < it.t1) {
                 const uint4(*from)[Q][G::ITEMS] = sm.raw[k % SEL_AHEAD];
-                float2 x[4], o[4], skip[4];
+                float2 x[4], o[4];
                 V::unpack(&from[0][0][tid], G::ITEMS, x);
-                param(1, skip);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = fma2(skip[e], x[e], sm.y[k & 1][tt][e * G::VECS + tid % G::VECS]);
                 const size_t at = (size_t)(it.row0 + t) * a.D + dv;
