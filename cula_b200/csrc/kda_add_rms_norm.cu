@@ -70,6 +70,17 @@ __device__ __forceinline__ int row_max(int v, int* slot) {
     return v;
 }
 
+// v / scale, as exact as a division: a product with the reciprocal alone is off by one and a half roundings, and puts twice as many values
+// on the other side of a boundary between two 8-bit values
+struct Quotient {
+    float scale, inv;
+    __device__ Quotient(float s) : scale(s < INFINITY ? s : 0.f), inv(1.f / s) {}    // by infinity: what is finite becomes zero
+    __device__ float2 of(float2 v) const {
+        const float2 q = mul2(v, splat2(inv));
+        return fma2(fma2(q, splat2(-scale), v), splat2(inv), q);
+    }
+};
+
 template <typename T, int RES, bool FP8, int TPR, int VPT>
 __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_kernel(const AddNormArgs a) {
     using R = typename StreamOf<RES, T>::type;
@@ -151,20 +162,22 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
                 if (a.group) {                                       // the threads of a group are neighbours in one warp
                     for (int o = a.group / 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
                     if (live && c < nv) {
-                        const float amax = __int_as_float(m) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax, inv = 1.f / scale;
+                        const float amax = __int_as_float(m) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax;
+                        const Quotient by(scale);
                         if (8 * c % a.group == 0) a.scale[row * (a.D / a.group) + 8 * c / a.group] = scale;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) val[v][e] = mul2(val[v][e], splat2(inv));
+                        for (int e = 0; e < 4; ++e) val[v][e] = by.of(val[v][e]);
                     }
                 } else top = max(top, m);
             }
             if (!a.group) {
-                const float amax = __int_as_float(row_max<TPR>(top, s_max[parity])) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax, inv = 1.f / scale;
+                const float amax = __int_as_float(row_max<TPR>(top, s_max[parity])) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax;
+                const Quotient by(scale);
                 if (live && lane == 0) a.scale[row] = scale;
 #pragma unroll
                 for (int v = 0; v < VPT; ++v)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) val[v][e] = mul2(val[v][e], splat2(inv));
+                    for (int e = 0; e < 4; ++e) val[v][e] = by.of(val[v][e]);
             }
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
