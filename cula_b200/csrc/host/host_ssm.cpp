@@ -4,6 +4,8 @@
 
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include "host_common.h"
 
@@ -72,6 +74,21 @@ void refuse_accumulators_of_the_default_stream(const Tensor& like) {
             if (const auto stream = edge.function->stream(); stream.has_value() && *stream == outside)
                 throw std::runtime_error("a backward pass cannot be captured while an earlier graph of the same leaves lives: its outputs hold their "
                                          "gradient accumulators, which belong to the default stream; let go of them first");
+}
+
+// Gradients that a graph is made of (create_graph) hang on the operator's inputs by a node that says that it cannot be differentiated:
+// left as constants, they would give second derivatives with a part missing.
+variable_list differentiable_once(variable_list grads) {
+    const auto node = torch::autograd::get_current_node();
+    if (!at::GradMode::is_enabled() || !node) return grads;
+    torch::autograd::edge_list inputs = node->next_edges();
+    const auto error = std::make_shared<torch::autograd::Error>("the gradients of this operator cannot be differentiated again", std::move(inputs));
+    for (Tensor& g : grads)
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::set_history(g, error);
+        }
+    return grads;
 }
 
 // ------------------------------------------------ selective scan ------------------------------------------------
@@ -159,11 +176,17 @@ cula_kda_selective_scan_args scan_args(const ScanInputs& in, const ScanSizes& s)
 struct ScanOutputs {
     Tensor y, hT, states, y_pre;
 };
+bool no_token(const ScanInputs& in) { return in.x.numel() == 0 || (in.tab && in.tab->total_tokens == 0); }
 ScanOutputs scan_forward(const ScanInputs& in, bool want_final, bool keep) {
     c10::cuda::CUDAGuard guard(in.x.device());
     const ScanSizes s = sizes_of(in);
     const auto f32 = in.A.options();
     ScanOutputs o;
+    if (no_token(in)) {                                              // the states stay what they were
+        o.y = at::zeros({s.B, s.T, s.D}, in.x.options());
+        if (want_final) o.hT = has(in.h0) ? in.h0->clone() : at::zeros({s.n_seqs, s.D, s.S}, f32);
+        return o;
+    }
     o.y = device_empty({s.B, s.T, s.D}, in.x.options());
     if (in.tab && in.tab->total_tokens < s.T) o.y.narrow(1, in.tab->total_tokens, s.T - in.tab->total_tokens).zero_();      // rows past the packed tokens
     if (want_final) o.hT = device_empty({s.n_seqs, s.D, s.S}, f32);
@@ -219,6 +242,12 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         const cudaStream_t stream = stream_of(in.x);
         const ScanSizes s = sizes_of(in);
         const auto f32 = in.A.options(), act = in.x.options();
+        if (no_token(in)) {
+            auto none = [&](const OptTensor& t) { return has(t) ? at::zeros(t->sizes(), t->options()) : Tensor(); };
+            const Tensor dh0 = !ctx->saved_data["h0"].toBool() ? Tensor() : dhT.defined() ? dhT.clone() : at::zeros({s.n_seqs, s.D, s.S}, f32);
+            return differentiable_once({none(in.x), none(in.dt), none(in.A), none(in.B), none(in.C), none(in.skip), none(in.z), none(in.bias), dh0,
+                                        Tensor(), Tensor(), Tensor()});
+        }
         Tensor dy;
         if (grads[0].defined()) {
             dy = grads[0].contiguous();
@@ -255,7 +284,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
             a.seg_dt = a.seg_state + n_seg * s.D * s.SP;
         }
         check(lib.cula_kda_selective_scan_bwd(&a, stream), "cula_kda_selective_scan_bwd");
-        return {dx, ddt, dA, dB, dC, dskip, dz, dbias, dh0, Tensor(), Tensor(), Tensor()};
+        return differentiable_once({dx, ddt, dA, dB, dC, dskip, dz, dbias, dh0, Tensor(), Tensor(), Tensor()});
     }
 };
 
@@ -302,11 +331,6 @@ std::pair<Tensor, OptTensor> selective_scan(const Tensor& x, const Tensor& dt, c
     }
     require(x.size(1) <= (int64_t)1 << 30 && x.size(0) <= (int64_t)1 << 30 && D <= (int64_t)1 << 24, "too many tokens or channels.");
     assert_blackwell(x);
-    if (x.numel() == 0 || (tab && tab->total_tokens == 0)) {         // no token: the states stay what they were
-        OptTensor fin;
-        if (want_final) fin = has(h0) ? h0->clone() : at::zeros({n_seqs, D, S}, x.options().dtype(at::kFloat).requires_grad(false));
-        return {at::zeros(x.sizes(), x.options().requires_grad(false)), fin};
-    }
     if (grad_wanted({x, dt, A, B, C, skip, z, bias, h0})) {
         auto out = SelectiveScan::apply(x, dt, A, B, C, skip, z, bias, h0, softplus, want_final, tab);
         return {out[0], out.size() > 1 ? OptTensor(out[1]) : OptTensor()};
@@ -332,7 +356,8 @@ OptTensor slots_of(const OptTensor& indices, const Tensor& x, int64_t rows, int6
     if (indices->dim() != 1 || indices->size(0) != rows || (indices->scalar_type() != at::kInt && indices->scalar_type() != at::kLong))
         throw pybind11::value_error(std::string(name) + " must hold one int32 slot per sequence");
     on_device_of(x, {{indices, name}});
-    return (indices->scalar_type() == at::kInt ? *indices : indices->to(at::kInt)).contiguous();
+    if (indices->scalar_type() == at::kInt) return indices->contiguous();
+    return indices->clamp(-1, INT_MAX).to(at::kInt).contiguous();            // what is past 32 bits is past the pool, not another slot
 }
 void check_out(const OptTensor& out, const Tensor& x) {
     if (!has(out)) return;
@@ -483,14 +508,14 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         Tensor dx = device_empty(v.sizes(), v.options().dtype(x_type)), dr;
         if (res && v.scalar_type() != x_type) dr = device_empty(v.sizes(), v.options());
         Tensor dw = device_empty({D}, w.options());
-        if (R == 0) return {dx, res ? (dr.defined() ? dr : dx) : Tensor(), dw.zero_().view(w.sizes()), Tensor()};
+        if (R == 0) return differentiable_once({dx, res ? (dr.defined() ? dr : dx) : Tensor(), dw.zero_(), Tensor()});
         Tensor part = device_empty({lib.cula_kda_add_rms_norm_shares((int)D, R), D}, w.options());
         cula_kda_add_rms_norm_args a{};
         a.v = ptr(v); a.w = fptr(w); a.rstd = fptr(rstd); a.dy = ptr(dy); a.dr_out = ptr(dr_out); a.dx = ptr(dx); a.dr = ptr(dr);
         a.part_w = fptr(part); a.dw = fptr(dw); a.R = R; a.D = (int)D; a.x_row = res ? D : row_stride(v);
         a.fp32 = x_type == at::kFloat; a.res = (int)res;
         check(lib.cula_kda_add_rms_norm_bwd(&a, stream_of(v)), "cula_kda_add_rms_norm_bwd");
-        return {dx, res ? (dr.defined() ? dr : dx) : Tensor(), dw, Tensor()};
+        return differentiable_once({dx, res ? (dr.defined() ? dr : dx) : Tensor(), dw, Tensor()});
     }
 };
 

@@ -61,7 +61,7 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
     x: ``[..., D]`` bf16 or fp32, D a multiple of 8 up to 16384; weight: ``[D]``; residual: the stream that the block adds to, of the
     shape of x, in fp32 or in the type of x, or None (then ``v`` is x itself). ``v`` has the residual's type, to which the sum is
     rounded once before it is normalised; ``y`` has the type of x. Gradients flow to x, residual and weight from both results, the
-    same from run to run."""
+    same from run to run; they cannot be differentiated again."""
     y, v = _native.host().add_rms_norm(x, weight, residual, eps)
     return y, x if v is None else v
 

@@ -23,8 +23,9 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     sequence; with ``output_final_state`` the states after the last tokens are returned, of a sequence without tokens the one before.
     Rows of a packed batch past its last token have zero outputs and gradients. States and sums are fp32.
 
-    Returns ``(y, final_state)``, y in the type of x. Gradients flow from both to every tensor argument and are the same from run to
-    run; a forward call that gradients will be asked of keeps the states before every eighth token (fp32)."""
+    Returns ``(y, final_state)``, y in the type of x. Gradients flow from both to every tensor argument, are the same from run to
+    run and cannot be differentiated again; a forward call that gradients will be asked of keeps the states before every eighth
+    token (fp32)."""
     tab = None if cu_seqlens is None else get_varlen_tables(cu_seqlens, cu_seqlens_cpu).native
     return _native.host().selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, tab)
 

@@ -135,6 +135,20 @@ def test_norm_with_one_gradient_only_and_views():
 
 
 @pytest.mark.gpu
+def test_norm_gradients_of_no_rows_and_not_differentiated_again():
+    from cula_b200.kda import add_rms_norm
+    x, w, r = (t.cuda().requires_grad_(True) for t in norm_inputs(5, 96, "bf16", "fp32"))
+    y, v = add_rms_norm(x[:0], w, r[:0])
+    for leaf, g in zip((x, w, r), torch.autograd.grad([y.sum(), v.sum()], [x, w, r])):
+        assert g.dtype == leaf.dtype and torch.equal(g, torch.zeros_like(leaf))
+    y, v = add_rms_norm(x, w, r)
+    gx, gw = torch.autograd.grad(y.float().square().sum(), [x, w], create_graph=True)
+    for g in (gx, gw):
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("R,D,dtype,res,group", [(*n, g) for n in NORMS for g in (None, 32, 128, 256) if g is None or n[1] % g == 0])
 def test_norm_in_8_bits(R, D, dtype, res, group):
     from cula_b200.kda import add_rms_norm_fp8

@@ -240,6 +240,35 @@ def test_no_tokens():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,cu,n", [(0, None, 2), (5, [0, 0, 0], 2), (5, [0], 0)])
+def test_gradients_of_no_tokens(T, cu, n):
+    """They are zeros, and the one of the first states is that of the last."""
+    from cula_b200.kda import selective_scan
+    a = on_gpu(make(2 if cu is None else 1, T, 16, 4, h0=2), grad=True)
+    a["initial_state"] = torch.randn(n, 16, 4, device="cuda", requires_grad=True)
+    y, fin = selective_scan(**a, output_final_state=True, cu_seqlens=None if cu is None else torch.tensor(cu, dtype=torch.int32, device="cuda"))
+    assert torch.equal(fin, a["initial_state"]) and (y == 0).all()
+    dfin = torch.randn_like(fin)
+    names = [k for k, v in a.items() if torch.is_tensor(v)]
+    for k, g in zip(names, torch.autograd.grad([y, fin], [a[k] for k in names], [torch.ones_like(y), dfin])):
+        assert g.shape == a[k].shape and g.dtype == a[k].dtype
+        assert torch.equal(g, dfin if k == "initial_state" else torch.zeros_like(a[k])), k
+
+
+@pytest.mark.gpu
+def test_gradients_are_not_differentiated_again():
+    from cula_b200.kda import selective_scan
+    a = on_gpu(make(1, 9, 16, 4, dtype=torch.float32), grad=True)
+    plain = torch.autograd.grad(selective_scan(**a)[0].square().sum(), [a["x"], a["A"]])
+    gx, gA = torch.autograd.grad(selective_scan(**a)[0].square().sum(), [a["x"], a["A"]], create_graph=True)
+    assert torch.equal(gx, plain[0]) and torch.equal(gA, plain[1])
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        torch.autograd.grad(gx.sum(), a["x"])
+    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+        torch.autograd.grad((gA * a["A"]).sum(), a["A"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_views_are_read_in_place_or_copied(dtype):
     """Parts of wider rows, broadcast rows, misaligned views: the same values as contiguous tensors, gradients in the views' shape."""
@@ -498,6 +527,22 @@ def test_step_slot_past_the_pool_is_reported():
     with pytest.raises(RuntimeError, match="past the end of the pool"):
         check_status(torch.device("cuda", 0))
     check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.gpu
+def test_step_slots_past_32_bits_name_no_other_slot():
+    from cula_b200.kda import check_status, selective_scan_update
+    a = on_gpu(make(3, 1, 16, 4))
+    pool = torch.randn(3, 16, 4, device="cuda")
+    before = pool.clone()
+    y = selective_scan_update(a["x"], a["dt"], a["A"], a["B"], a["C"], pool, state_indices=torch.tensor([2 ** 32, 2, 2 - 2 ** 32], device="cuda"))
+    torch.cuda.synchronize()
+    assert (y[[0, 2]] == 0).all() and torch.equal(pool[:2], before[:2])
+    want = before[2:].clone()
+    selective_scan_update(a["x"][1:2], a["dt"][1:2], a["A"], a["B"][1:2], a["C"][1:2], want)
+    assert torch.equal(pool[2:], want)
+    with pytest.raises(RuntimeError, match="past the end of the pool"):
+        check_status(torch.device("cuda", 0))
 
 
 @pytest.mark.gpu
