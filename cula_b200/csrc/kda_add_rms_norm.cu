@@ -70,15 +70,12 @@ __device__ __forceinline__ int row_max(int v, int* slot) {
     return v;
 }
 
-// v / scale, as exact as a division: a product with the reciprocal alone is off by one and a half roundings, and puts twice as many values
-// on the other side of a boundary between two 8-bit values
+// v / scale, as exact as a division: a product with the reciprocal alone is off by a rounding more, and puts twice as many values on the
+// other side of a boundary between two 8-bit values. The reciprocal has a second part, its own rounding.
 struct Quotient {
-    float scale, inv;
-    __device__ Quotient(float s) : scale(s < INFINITY ? s : 0.f), inv(1.f / s) {}    // by infinity: what is finite becomes zero
-    __device__ float2 of(float2 v) const {
-        const float2 q = mul2(v, splat2(inv));
-        return fma2(fma2(q, splat2(-scale), v), splat2(inv), q);
-    }
+    float inv, rest;
+    __device__ Quotient(float scale) : inv(1.f / scale), rest(scale < INFINITY ? fmaf(-scale, inv, 1.f) * inv : 0.f) {}
+    __device__ float2 of(float2 v) const { return fma2(v, splat2(inv), mul2(v, splat2(rest))); }
 };
 
 template <typename T, int RES, bool FP8, int TPR, int VPT>
