@@ -4,7 +4,7 @@
 //     dv = rstd (dn - n mean(dn n)) + dr_out with dn = dy w;  dx, dr = dv;  dw = sum over rows of dy n
 // Everything is read and written once: TPR threads hold a row in registers, VPT pieces of 8 columns each, and ask for their next row before
 // they sum, scale and store this one. Bound by memory: 8192 x 4096 in bf16 forward 40 us (268 MB: 6.6 TB/s), backward 44 (268 MB), 8-bit output
-// beside an fp32 stream at 16384 x 4096 112 us (738 MB: 6.6 TB/s).
+// beside an fp32 stream at 16384 x 4096 112 us (738 MB: 6.6 TB/s), 114 with a scale per 128 columns.
 #include <cuda_fp8.h>
 
 #include "kda_common.cuh"
@@ -130,7 +130,6 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
         fetch(row + step);                                           // on its way while this row is summed, scaled and stored
         const float rstd = rsqrtf(row_sum<TPR>(ss.x + ss.y, s_sum[parity]) * (1.f / a.D) + a.eps);
         if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
-        int top = 0;                                                 // bits of the largest |y|: a NaN is larger than anything
 #pragma unroll
         for (int v = 0; v < VPT; ++v) {
             const int c = lane + v * TPR;
@@ -148,27 +147,40 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
             }
         }
         if constexpr (FP8) {
+            int m[VPT];                                              // bits of the largest |y| of a piece: a NaN is larger than anything
 #pragma unroll
             for (int v = 0; v < VPT; ++v) {
-                const int c = lane + v * TPR;
-                int m = 0;
-                if (live && c < nv) {
+                m[v] = 0;
+                if (live && lane + v * TPR < nv) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) m = max(m, max(__float_as_int(fabsf(val[v][e].x)), __float_as_int(fabsf(val[v][e].y))));
+                    for (int e = 0; e < 4; ++e) m[v] = max(m[v], max(__float_as_int(fabsf(val[v][e].x)), __float_as_int(fabsf(val[v][e].y))));
                 }
-                if (a.group) {                                       // the threads of a group are neighbours in one warp
-                    for (int o = a.group / 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            }
+            auto scale_of = [](int bits) {
+                const float s = __int_as_float(bits) / E4M3_MAX;
+                return s < SCALE_MIN ? SCALE_MIN : s;
+            };
+            if (a.group) {                                           // the threads of a group are neighbours in one warp
+                for (int o = a.group / 16; o; o >>= 1)
+#pragma unroll
+                    for (int v = 0; v < VPT; ++v) m[v] = max(m[v], __shfl_xor_sync(0xffffffffu, m[v], o));
+                const int pieces = 31 - __clz(a.group / 8);          // log2 of a group's threads
+#pragma unroll
+                for (int v = 0; v < VPT; ++v) {
+                    const int c = lane + v * TPR;
                     if (live && c < nv) {
-                        const float amax = __int_as_float(m) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax;
+                        const float scale = scale_of(m[v]);
                         const Quotient by(scale);
-                        if (8 * c % a.group == 0) a.scale[row * (a.D / a.group) + 8 * c / a.group] = scale;
+                        if (c == c >> pieces << pieces) a.scale[row * (nv >> pieces) + (c >> pieces)] = scale;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) val[v][e] = by.of(val[v][e]);
                     }
-                } else top = max(top, m);
-            }
-            if (!a.group) {
-                const float amax = __int_as_float(row_max<TPR>(top, s_max[parity])) / E4M3_MAX, scale = amax < SCALE_MIN ? SCALE_MIN : amax;
+                }
+            } else {
+                int top = m[0];
+#pragma unroll
+                for (int v = 1; v < VPT; ++v) top = max(top, m[v]);
+                const float scale = scale_of(row_max<TPR>(top, s_max[parity]));
                 const Quotient by(scale);
                 if (live && lane == 0) a.scale[row] = scale;
 #pragma unroll
