@@ -38,14 +38,14 @@ template <int RES, typename T> struct StreamOf { using type = T; };
 template <typename T> struct StreamOf<RES_BF16, T> { using type = __nv_bfloat16; };
 template <typename T> struct StreamOf<RES_FP32, T> { using type = float; };
 
-constexpr int norm_threads(int TPR) { return TPR < 128 ? 128 : TPR; }
+constexpr int norm_threads(int TPR) { return TPR < 64 ? 128 : TPR; }
 
-// the sum (or the maximum of bit patterns) over the TPR threads of a row; `slot` is theirs for this call and not written again before
-// another barrier has passed
+// the sum (or the maximum of bit patterns) over the TPR threads of a row, a part of a warp or whole warps; `slot` is theirs for this call and
+// not written again before another barrier has passed
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* slot) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (TPR > 32) {
         const int warp = threadIdx.x >> 5;
         if ((threadIdx.x & 31) == 0) slot[warp] = v;
@@ -58,7 +58,10 @@ __device__ __forceinline__ float row_sum(float v, float* slot) {
 }
 template <int TPR>
 __device__ __forceinline__ int row_max(int v, int* slot) {
-    v = __reduce_max_sync(0xffffffffu, v);
+    if constexpr (TPR < 32) {
+#pragma unroll
+        for (int o = TPR / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    } else v = __reduce_max_sync(0xffffffffu, v);
     if constexpr (TPR > 32) {
         const int warp = threadIdx.x >> 5;
         if ((threadIdx.x & 31) == 0) slot[warp] = v;
@@ -78,10 +81,15 @@ struct Quotient {
     __device__ float2 of(float2 v) const { return fma2(v, splat2(inv), mul2(v, splat2(rest))); }
 };
 
+// Blocks that an SM holds where the registers allow it: of the rows that are on their way, the narrow ones are the fewest bytes
+// (4096 x 8192 in bf16, no residual: 36 -> 30 us)
+constexpr int norm_fwd_blocks(int RES, bool FP8, bool fp32, int TPR, int VPT) {
+    return TPR == 512 && VPT == 2 && !fp32 && (RES == RES_NONE || (RES == RES_BF16 && !FP8)) ? 2 : 1;
+}
 template <typename T, int RES, bool FP8, int TPR, int VPT>
-__global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_kernel(const AddNormArgs a) {
+__global__ void __launch_bounds__(norm_threads(TPR), norm_fwd_blocks(RES, FP8, sizeof(T) == 4, TPR, VPT)) kda_add_rms_norm_fwd_kernel(const AddNormArgs a) {
     using R = typename StreamOf<RES, T>::type;
-    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR < 32 ? 1 : TPR / 32;
+    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR <= 32 ? 1 : TPR / 32;
     __shared__ float s_sum[2][WARPS];
     __shared__ int s_max[2][WARPS];
     const int lane = threadIdx.x % TPR, nv = a.D / 8;
@@ -202,11 +210,13 @@ __global__ void __launch_bounds__(norm_threads(TPR), 1) kda_add_rms_norm_fwd_ker
     }
 }
 
-// (two rows' loads of two pieces per thread fit 128 registers, so that an SM holds 512 threads: 60 -> 45 us at 8192 x 4096)
+// Blocks that an SM holds: two rows' loads of two pieces per thread fit 128 registers, so that there are 512 threads (60 -> 45 us at 8192 x 4096);
+// those of one piece fit 64, or 100 in fp32
+constexpr int norm_bwd_resident(bool fp32, int TPR, int VPT) { return (VPT == 2 ? 512 : fp32 ? 640 : 1024) / norm_threads(TPR); }
 template <typename T, int RES, int TPR, int VPT>
-__global__ void __launch_bounds__(norm_threads(TPR), TPR > 32 && VPT == 2 ? 512 / norm_threads(TPR) : 1) kda_add_rms_norm_bwd_kernel(const AddNormArgs a) {
+__global__ void __launch_bounds__(norm_threads(TPR), norm_bwd_resident(RES == RES_FP32 || sizeof(T) == 4, TPR, VPT)) kda_add_rms_norm_bwd_kernel(const AddNormArgs a) {
     using R = typename StreamOf<RES, T>::type;
-    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR < 32 ? 1 : TPR / 32;
+    constexpr int GROUPS = norm_threads(TPR) / TPR, WARPS = TPR <= 32 ? 1 : TPR / 32;
     __shared__ float s_sum[2][WARPS];
     const int lane = threadIdx.x % TPR, nv = a.D / 8;
     const long long group = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR;
@@ -249,7 +259,6 @@ __global__ void __launch_bounds__(norm_threads(TPR), TPR > 32 && VPT == 2 ? 512 
             const int c = lane + v * TPR;
             if (live && c < nv) {
                 float2 dy[4], wv[4];
-                if constexpr (TPR * VPT > 1024) w[v].load(a.w + 8 * c);          // too many to be held
                 w[v].get(wv);
                 rv[v].get(n[v]);
                 ry[v].get(dy);
@@ -321,6 +330,86 @@ __global__ void __launch_bounds__(norm_threads(TPR), TPR > 32 && VPT == 2 ? 512 
     }
 }
 
+// Rows that registers do not hold (D > 8192) are read once for the sum and once more, out of L2, for the gradients: 2730 x 12288 beside an fp32
+// stream takes 112 us (floor 83), and 287 with a thousand bytes of spilled registers per thread
+template <typename T, int RES, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR, 2) kda_add_rms_norm_bwd_wide_kernel(const AddNormArgs a) {
+    using R = typename StreamOf<RES, T>::type;
+    __shared__ float s_sum[2][TPR / 32];
+    const int lane = threadIdx.x, nv = a.D / 8;
+    pdl_launch_dependents();
+    pdl_wait();
+    float2 dw[VPT][4];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dw[v][e] = make_float2(0.f, 0.f);
+    int parity = 0;
+    for (long long row = blockIdx.x; row < a.R; row += gridDim.x, parity ^= 1) {
+        const R* vp = static_cast<const R*>(a.v) + (RES == RES_NONE ? row * a.x_row : row * a.D);
+        const T* yp = static_cast<const T*>(a.dy) + row * a.D;
+        const float rstd = a.rstd[row];
+        auto piece = [&](int c, float2 (&n)[4], float2 (&dy)[4], float2 (&dn)[4]) {
+            Oct<R> rv;
+            Oct<T> ry;
+            Oct<float> rw;
+            rv.load(vp + 8 * c);
+            ry.load(yp + 8 * c);
+            rw.load(a.w + 8 * c);
+            rv.get(n);
+            ry.get(dy);
+            rw.get(dn);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                n[e] = mul2(n[e], splat2(rstd));
+                dn[e] = mul2(dy[e], dn[e]);
+            }
+        };
+        float2 dot = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+            if (const int c = lane + v * TPR; c < nv) {
+                float2 n[4], dy[4], dn[4];
+                piece(c, n, dy, dn);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dot = fma2(dn[e], n[e], dot);
+            }
+        const float m = -row_sum<TPR>(dot.x + dot.y, s_sum[parity]) * (1.f / a.D);
+#pragma unroll
+        for (int v = 0; v < VPT; ++v)
+            if (const int c = lane + v * TPR; c < nv) {
+                const size_t at = (size_t)row * a.D + 8 * c;
+                float2 n[4], dy[4], dn[4], d[4];
+                if (RES != RES_NONE && a.dr_out) {
+                    Oct<R> rd;
+                    rd.load(static_cast<const R*>(a.dr_out) + at);
+                    rd.get(d);
+                } else d[0] = d[1] = d[2] = d[3] = make_float2(0.f, 0.f);
+                piece(c, n, dy, dn);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dw[v][e] = fma2(dy[e], n[e], dw[v][e]);
+                    d[e] = fma2(splat2(rstd), fma2(n[e], splat2(m), dn[e]), d[e]);
+                }
+                Oct<T> ox;
+                ox.set(d);
+                ox.store(static_cast<T*>(a.dx) + at);
+                if (RES != RES_NONE && a.dr) {
+                    Oct<R> orr;
+                    orr.set(d);
+                    orr.store(static_cast<R*>(a.dr) + at);
+                }
+            }
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+        if (const int c = lane + v * TPR; c < nv) {
+            Oct<float> o;
+            o.set(dw[v]);
+            o.store(a.part_w + (size_t)blockIdx.x * a.D + 8 * c);
+        }
+}
+
 // the shares of dw added up in a fixed order: 32 columns per block, 32 threads to a column
 __global__ void __launch_bounds__(1024) kda_add_rms_norm_sum_kernel(const float* part, float* dw, int D, int rows) {
     __shared__ float s[32][33];
@@ -343,47 +432,50 @@ __global__ void __launch_bounds__(1024) kda_add_rms_norm_sum_kernel(const float*
 // Threads and pieces for a row: a warp up to 1024 columns, two pieces per thread above that. Where rows are few, one piece per thread
 // (forward): a row's latency is then the call's.
 struct NormShape { int tpr, vpt; };
+// As many threads as a row has pieces, or pairs of pieces: idle ones cost loads that could be on their way (2560 columns, backward, fp32 stream:
+// 113 -> 101 us with 160 threads in the place of 256; 64 columns 182 -> 93 with 8 in the place of 32)
 static NormShape norm_shape(int D, long long R, bool backward) {
     const int nv = D / 8;
-    if (nv <= 32) return {32, 1};
-    if (nv <= 64) return {32, 2};
-    if (nv <= 128) return {32, 4};
+    if (nv <= 32) return {nv <= 8 ? 8 : nv <= 16 ? 16 : 32, 1};
+    if (backward && nv <= 128) return {nv <= 64 ? 64 : nv <= 96 ? 96 : 128, 1};
+    if (nv <= 128) return {32, nv <= 64 ? 2 : 4};
     if (nv <= 512 && R <= 2LL * sm_count() && !backward) return {512, 1};
-    if (nv <= 256) return {128, 2};
-    if (nv <= 512) return {256, 2};
-    if (nv <= 1024) return {512, 2};
-    return {512, 4};
+    if (nv <= 768) return {nv <= 256 ? 128 : nv <= 320 ? 160 : nv <= 384 ? 192 : nv <= 512 ? 256 : nv <= 640 ? 320 : 384, 2};
+    return {512, nv <= 1024 ? 2 : 4};
 }
-// f<TPR, VPT>() for a shape
+// f<TPR, VPT>() for a shape of either direction
 #define KDA_NORM_SHAPES(s, KERNEL)                                                                                              \
-    ((s).tpr == 32 ? ((s).vpt == 1 ? KERNEL(32, 1) : (s).vpt == 2 ? KERNEL(32, 2) : KERNEL(32, 4))                                  \
-     : (s).tpr == 128 ? KERNEL(128, 2) : (s).tpr == 256 ? KERNEL(256, 2)                                                          \
-     : (s).vpt == 1 ? KERNEL(512, 1) : (s).vpt == 2 ? KERNEL(512, 2) : KERNEL(512, 4))
+    ((s).tpr == 8 ? KERNEL(8, 1) : (s).tpr == 16 ? KERNEL(16, 1)                                                                    \
+     : (s).tpr == 128 ? KERNEL(128, 2) : (s).tpr == 160 ? KERNEL(160, 2) : (s).tpr == 192 ? KERNEL(192, 2)                          \
+     : (s).tpr == 256 ? KERNEL(256, 2) : (s).tpr == 320 ? KERNEL(320, 2) : (s).tpr == 384 ? KERNEL(384, 2) : KERNEL(512, 2))
 
 template <typename T, int RES, bool FP8>
 static int launch_norm_fwd(const AddNormArgs& a, cudaStream_t stream) {
     const NormShape s = norm_shape(a.D, a.R, false);
 #define KDA_NORM_FWD(TPR, VPT) kda_add_rms_norm_fwd_kernel<T, RES, FP8, TPR, VPT>
-    void (*kernel)(const AddNormArgs) = KDA_NORM_SHAPES(s, KDA_NORM_FWD);
+    void (*kernel)(const AddNormArgs) = s.tpr == 32 ? (s.vpt == 1 ? KDA_NORM_FWD(32, 1) : s.vpt == 2 ? KDA_NORM_FWD(32, 2) : KDA_NORM_FWD(32, 4))
+                                        : s.tpr == 512 && s.vpt != 2 ? (s.vpt == 1 ? KDA_NORM_FWD(512, 1) : KDA_NORM_FWD(512, 4))
+                                                                     : KDA_NORM_SHAPES(s, KDA_NORM_FWD);
 #undef KDA_NORM_FWD
     const int threads = norm_threads(s.tpr), groups = threads / s.tpr;
     const long long want = (a.R + groups - 1) / groups, cap = sm_count() * (2048LL / threads);
     return (int)launch_early(kernel, dim3((unsigned)(want < cap ? want : cap)), threads, 0, stream, a);
 }
-static long long norm_bwd_blocks(int D, long long R, NormShape s) {
+static long long norm_bwd_blocks(int D, long long R, bool fp32, NormShape s) {
     const int groups = norm_threads(s.tpr) / s.tpr;
-    const long long want = (R + groups - 1) / groups, cap = sm_count() * (s.tpr == 512 ? 1LL : s.tpr == 256 ? 2LL : 4LL);
+    const long long want = (R + groups - 1) / groups, cap = (long long)sm_count() * (s.vpt == 4 ? 2 : norm_bwd_resident(fp32, s.tpr, s.vpt));
     return want < cap ? want : cap;
 }
 template <typename T, int RES>
 static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
     const NormShape s = norm_shape(a.D, a.R, true);
 #define KDA_NORM_BWD(TPR, VPT) kda_add_rms_norm_bwd_kernel<T, RES, TPR, VPT>
-    void (*kernel)(const AddNormArgs) = KDA_NORM_SHAPES(s, KDA_NORM_BWD);
+    void (*kernel)(const AddNormArgs) = s.vpt == 4 ? kda_add_rms_norm_bwd_wide_kernel<T, RES, 512, 4> : s.tpr == 32 ? KDA_NORM_BWD(32, 1)
+                                        : s.tpr == 64 ? KDA_NORM_BWD(64, 1) : s.tpr == 96 ? KDA_NORM_BWD(96, 1)
+                                        : s.vpt == 1 && s.tpr == 128 ? KDA_NORM_BWD(128, 1) : KDA_NORM_SHAPES(s, KDA_NORM_BWD);
 #undef KDA_NORM_BWD
-    const int threads = norm_threads(s.tpr);
-    const long long blocks = norm_bwd_blocks(a.D, a.R, s);
-    if (const cudaError_t e = launch_early(kernel, dim3((unsigned)blocks), threads, 0, stream, a); e != cudaSuccess) return (int)e;
+    const long long blocks = norm_bwd_blocks(a.D, a.R, RES == RES_FP32 || sizeof(T) == 4, s);
+    if (const cudaError_t e = launch_early(kernel, dim3((unsigned)blocks), norm_threads(s.tpr), 0, stream, a); e != cudaSuccess) return (int)e;
     return (int)launch_early(kda_add_rms_norm_sum_kernel, dim3((a.D + 31) / 32), 1024, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)blocks);
 }
 
@@ -393,7 +485,7 @@ static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
 extern "C" int kda_add_rms_norm_shares(int D, long long R) {
     using namespace kda;
     const NormShape s = norm_shape(D, R, true);
-    return (int)norm_bwd_blocks(D, R, s);
+    return (int)norm_bwd_blocks(D, R, false, s);                     // of the type that takes the most
 }
 
 extern "C" int kda_launch_add_rms_norm(const kda::AddNormArgs* a, int backward, cudaStream_t stream) {

@@ -73,7 +73,9 @@ def test_refusals():
 # ------------------------------------------------ residual RMS norm ------------------------------------------------
 NORMS = [(1, 8, "bf16", "bf16"), (5, 64, "fp32", "fp32"), (3, 264, "bf16", "fp32"), (33, 520, "bf16", "none"), (7, 1000, "fp32", "none"), (333, 1024, "bf16", "bf16"),
          (2, 1032, "bf16", "bf16"), (400, 2056, "bf16", "fp32"), (5, 4096, "bf16", "bf16"), (310, 4096, "fp32", "fp32"), (9, 4104, "bf16", "none"), (6, 8192, "fp32", "fp32"),
-         (3, 16384, "bf16", "fp32"), (2, 12288, "fp32", "none")]
+         (3, 16384, "bf16", "fp32"), (2, 12288, "fp32", "none"),
+         (35, 128, "bf16", "bf16"), (40, 72, "fp32", "fp32"), (33, 136, "bf16", "none"), (9, 512, "bf16", "fp32"), (11, 768, "fp32", "fp32"), (400, 2560, "bf16", "bf16"),
+         (5, 2568, "fp32", "none"), (301, 5120, "bf16", "fp32"), (4, 6144, "bf16", "none"), (300, 8192, "bf16", "bf16"), (301, 8200, "bf16", "bf16")]
 
 
 def norm_inputs(R, D, dtype, res, seed=0):
