@@ -32,20 +32,38 @@ __device__ __forceinline__ float4 step_four(const T* row, int n, int S, int vec)
     r.w = n + 3 < S ? step_load(row + n + 3) : 0.f;
     return r;
 }
-// the same as they are, to be converted when they are needed
-template <typename T>
-__device__ __forceinline__ void step_raw4(T (&v)[4], const T* row, int n, int S, int vec) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec) {
-            const uint2 r = n < S ? *reinterpret_cast<const uint2*>(row + n) : make_uint2(0u, 0u);
-            *reinterpret_cast<uint32_t*>(&v[0]) = r.x;
-            *reinterpret_cast<uint32_t*>(&v[2]) = r.y;
-            return;
+// Values as they are, to be converted when they are needed: whatever is done to them where they are loaded, taking a word apart among it,
+// waits for the load (256 rows x 4096 channels x 8 states in bf16: 27 us so, 20 without)
+__device__ __forceinline__ uint32_t step_raw(const float* p) { return *reinterpret_cast<const uint32_t*>(p); }
+__device__ __forceinline__ uint32_t step_raw(const __nv_bfloat16* p) { return *reinterpret_cast<const unsigned short*>(p); }
+template <typename T> __device__ __forceinline__ float step_value(uint32_t r) { return __uint_as_float(sizeof(T) == 2 ? r << 16 : r); }
+template <typename T> struct Raw4 {                                 // four values: two words of bf16, four of fp32
+    uint32_t v[sizeof(T)];
+    __device__ __forceinline__ void load(const T* row, int n, int S, int vec) {
+        if constexpr (sizeof(T) == 2) {
+            if (vec) {
+                const uint2 r = n < S ? *reinterpret_cast<const uint2*>(row + n) : make_uint2(0u, 0u);
+                v[0] = r.x; v[1] = r.y;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    v[k] = (n + 2 * k < S ? step_raw(row + n + 2 * k) : 0u) | (n + 2 * k + 1 < S ? step_raw(row + n + 2 * k + 1) : 0u) << 16;
+            }
+        } else if (vec) {
+            const uint4 r = n < S ? *reinterpret_cast<const uint4*>(row + n) : make_uint4(0u, 0u, 0u, 0u);
+            v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = n + k < S ? step_raw(row + n + k) : 0u;
         }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = n + k < S ? row[n + k] : T(0.f);
-}
+    __device__ __forceinline__ float4 get() const {
+        if constexpr (sizeof(T) == 2) {
+            const float2 a = unpack_bf16(v[0]), b = unpack_bf16(v[1]);
+            return make_float4(a.x, a.y, b.x, b.y);
+        } else return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+    }
+};
 // the pool slot of a row, or -1
 __device__ __forceinline__ int step_slot(const int* indices, int row, int pool, int* status) {
     if (!indices) return row;
@@ -64,9 +82,11 @@ __device__ __forceinline__ int step_slot(const int* indices, int row, int pool, 
 // and 28.8 so (5.0 TB/s, launch and ramp included; 512 rows 5.3). One row ahead in registers: 29.3, and 46 in the place of 28 where 64
 // states leave none. A ring of 2 or 4 rows: 33, 35.
 constexpr int STEP_RING = 3;
+// Blocks that an SM holds: those of few states per channel need more of them for as many bytes on their way (8 states: 23 -> 19 us)
+constexpr int step_resident(int SL) { return SL == 1 ? 8 : SL == 2 ? 6 : 5; }
 
 template <int SL, typename T>
-__global__ void __launch_bounds__(STEP_THREADS) kda_selective_step_kernel(const SelStepArgs a, const int tiles, const int row_step) {
+__global__ void __launch_bounds__(STEP_THREADS, step_resident(SL)) kda_selective_step_kernel(const SelStepArgs a, const int tiles, const int row_step) {
     constexpr int CG = 32 / SL, NI = SL < 4 ? SL : 4, SHARE = SL / NI;      // SHARE: lanes that are left with a channel's sum
     __shared__ float4 ring[STEP_RING][NI][STEP_THREADS];
     const int tid = threadIdx.x, lane = tid & 31, s = lane % SL, g = lane / SL, n0 = 4 * s, c_own = s / SHARE;
@@ -100,15 +120,16 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_selective_step_kernel(const 
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    T raw[3], Bn[4], Cn[4];                                          // x, dt, z, B, C of the row to come
+    uint32_t raw[3];
+    Raw4<T> Bn, Cn;                                                  // x, dt, z, B, C of the row to come
     auto fetch = [&](int r, int at) {
         if (at < 0) return;
-        raw[0] = static_cast<const T*>(a.x)[r * a.x_row + dm];
-        raw[1] = static_cast<const T*>(a.dt)[r * a.dt_row + dm];
-        if (a.z) raw[2] = static_cast<const T*>(a.z)[r * a.z_row + dm];
+        raw[0] = step_raw(static_cast<const T*>(a.x) + r * a.x_row + dm);
+        raw[1] = step_raw(static_cast<const T*>(a.dt) + r * a.dt_row + dm);
+        if (a.z) raw[2] = step_raw(static_cast<const T*>(a.z) + r * a.z_row + dm);
         if (one_group) {
-            step_raw4(Bn, static_cast<const T*>(a.Bm) + r * a.b_row + group0 * a.S, n0, a.S, a.vec);
-            step_raw4(Cn, static_cast<const T*>(a.Cm) + r * a.c_row + group0 * a.S, n0, a.S, a.vec);
+            Bn.load(static_cast<const T*>(a.Bm) + r * a.b_row + group0 * a.S, n0, a.S, a.vec);
+            Cn.load(static_cast<const T*>(a.Cm) + r * a.c_row + group0 * a.S, n0, a.S, a.vec);
         }
     };
     int row = blockIdx.x / tiles, slots[STEP_RING + 1];              // of this row and the ones to come
@@ -120,9 +141,8 @@ __global__ void __launch_bounds__(STEP_THREADS) kda_selective_step_kernel(const 
     for (int k = 0; row < a.rows; row += row_step, k = k + 1 == STEP_RING ? 0 : k + 1) {
         const int at = slots[0];
         fetch_state(k == 0 ? STEP_RING - 1 : k - 1, slots[STEP_RING - 1]);
-        const float4 B0 = make_float4(step_load(&Bn[0]), step_load(&Bn[1]), step_load(&Bn[2]), step_load(&Bn[3]));
-        const float4 C0 = make_float4(step_load(&Cn[0]), step_load(&Cn[1]), step_load(&Cn[2]), step_load(&Cn[3]));
-        const float x = step_load(&raw[0]), dt = step_load(&raw[1]) + bias, z = a.z ? step_load(&raw[2]) : 0.f;
+        const float4 B0 = Bn.get(), C0 = Cn.get();
+        const float x = step_value<T>(raw[0]), dt = step_value<T>(raw[1]) + bias, z = a.z ? step_value<T>(raw[2]) : 0.f;
 #pragma unroll
         for (int i = 0; i < STEP_RING; ++i) slots[i] = slots[i + 1];
         slots[STEP_RING] = slot_of(row + (STEP_RING + 1) * row_step);
@@ -270,7 +290,7 @@ static StepGrid step_grid(int rows, int units, int resident) {       // units: t
 template <int SL, typename T>
 static int launch_sel_step(const SelStepArgs& a, cudaStream_t stream) {
     constexpr int channels = 32 / SL * (SL < 4 ? SL : 4);            // of a warp
-    const StepGrid g = step_grid(a.rows, (a.D + channels - 1) / channels * 32, 5);
+    const StepGrid g = step_grid(a.rows, (a.D + channels - 1) / channels * 32, step_resident(SL));
     return (int)launch_early(kda_selective_step_kernel<SL, T>, dim3((unsigned)(g.tiles * g.row_step)), g.threads, 0, stream, a, g.tiles, g.row_step);
 }
 
