@@ -76,12 +76,12 @@ __device__ __forceinline__ int step_slot(const int* indices, int row, int pool, 
 }
 
 // SL lanes (four states each) share a channel, NI channels a lane: channel c of lane (g, s) is the warp's c (32 / SL) + g. What concerns a
-// channel as a whole (step, gate, output) is done by one lane, its owner, and handed to the others. The states of the next two rows are
-// on their way to shared memory, each thread's to a place of its own, while a row is worked on; everything else is asked for one row ahead.
+// channel as a whole (step, gate, output) is done by one lane, its owner, and handed to the others. The next row's states are on their way to
+// shared memory, each thread's to a place of its own, while a row is worked on; everything else is asked for one row ahead too.
 // Bound by memory: 256 rows x 4096 channels x 16 states in bf16 (143 MB, 22 us at the copy rate) take 65 us with a block per row and tile
-// and 28.8 so (5.0 TB/s, launch and ramp included; 512 rows 5.3). One row ahead in registers: 29.3, and 46 in the place of 28 where 64
-// states leave none. A ring of 2 or 4 rows: 33, 35.
-constexpr int STEP_RING = 3;
+// and 27.8 so (5.1 TB/s, launch and ramp included; 512 rows 5.6). The next row in registers: 29.3, and 46 in the place of 28 where 64 states
+// leave none. Two rows ahead: 28.6; other numbers of blocks per SM: 30 to 35.
+constexpr int STEP_RING = 2;
 // Blocks that an SM holds: those of few states per channel need more of them for as many bytes on their way (8 states: 23 -> 19 us)
 constexpr int step_resident(int SL) { return SL == 1 ? 8 : SL == 2 ? 6 : 5; }
 
