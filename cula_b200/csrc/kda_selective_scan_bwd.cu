@@ -28,7 +28,9 @@ __device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0
 template <int SL, typename T>
 struct SelBwdSmem {
     using G = SelShape<SL>;
-    static constexpr int Q = SelVec<T>::Q, RING = Q == 1 ? 3 : 2;    // tiles of rows: of the gradients that are made, of the next tile, one more of 16 bits
+    // tiles of rows: of the gradients that are made, of the next tile, one more of 16 bits where two CTAs still share an SM
+    // (64 states, 4 x 2048 x 4096: 2.88 ms with three, 2.13 with two)
+    static constexpr int Q = SelVec<T>::Q, RING = Q == 1 && SL < 16 ? 3 : 2;
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float2 dy[2][G::LC][G::CH / 2];
     float4 b[2][G::LC][SL], c[2][G::LC][SL];
@@ -43,6 +45,7 @@ struct SelBwdSmem {
     };
     static_assert(sizeof(acc) <= 2 * sizeof(kept), "");
 };
+static_assert(sizeof(SelBwdSmem<16, __nv_bfloat16>) <= 113 * 1024 && sizeof(SelBwdSmem<4, float>) <= 113 * 1024, "two CTAs per SM");
 
 // What the serving warps do for an item: rows of the tiles to come, operands of the next tile, gradients of the one before.
 template <int SL, typename T, bool STATE_ONLY>
@@ -410,12 +413,11 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                                 sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[0];
                             }
                         } else {
-                            constexpr int LEFT = 8 / CL;
-#pragma unroll
-                            for (int k = 0; k < LEFT; ++k) {
-                                const int id = cl * LEFT + k;
-                                sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)] = r[k];
-                            }
+                            constexpr int LEFT = 8 / CL;         // neighbours
+                            const int id = cl * LEFT;
+                            float* to = &sm.bc[buf][warp][tb + u][(id >> 2) * SP + n0 + (id & 3)];
+                            if constexpr (LEFT == 4) *reinterpret_cast<float4*>(to) = make_float4(r[0], r[1], r[2], r[3]);
+                            else *reinterpret_cast<float2*>(to) = make_float2(r[0], r[1]);
                         }
                     }
                 }
