@@ -410,23 +410,27 @@ __global__ void __launch_bounds__(TPR, 2) kda_add_rms_norm_bwd_wide_kernel(const
         }
 }
 
-// the shares of dw added up in a fixed order: 32 columns per block, 32 threads to a column
+// the shares of dw added up in a fixed order: 32 columns per block with 32 threads each, or 8 with 128 where 32 would leave SMs without a block
+template <int COLS>
 __global__ void __launch_bounds__(1024) kda_add_rms_norm_sum_kernel(const float* part, float* dw, int D, int rows) {
-    __shared__ float s[32][33];
-    const int lane = threadIdx.x & 31, k0 = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    __shared__ float s[32][COLS + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * COLS + threadIdx.x % COLS;
     pdl_launch_dependents();
     pdl_wait();
     float sum = 0.f;
     if (col < D) {
 #pragma unroll 8
-        for (int k = k0; k < rows; k += 32) sum += part[(size_t)k * D + col];
+        for (int k = threadIdx.x / COLS; k < rows; k += 1024 / COLS) sum += part[(size_t)k * D + col];
     }
-    s[k0][lane] = sum;
+#pragma unroll
+    for (int o = COLS; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < COLS) s[warp][lane] = sum;
     __syncthreads();
-    sum = s[lane][k0];                                               // a warp per column
+    if (warp >= COLS) return;
+    sum = s[lane][warp];                                             // a warp per column
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0 && blockIdx.x * 32 + k0 < D) dw[blockIdx.x * 32 + k0] = sum;
+    if (lane == 0 && blockIdx.x * COLS + warp < D) dw[blockIdx.x * COLS + warp] = sum;
 }
 
 // Threads and pieces for a row: a warp up to 1024 columns, two pieces per thread above that. Where rows are few, one piece per thread
@@ -476,7 +480,8 @@ static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
 #undef KDA_NORM_BWD
     const long long blocks = norm_bwd_blocks(a.D, a.R, RES == RES_FP32 || sizeof(T) == 4, s);
     if (const cudaError_t e = launch_early(kernel, dim3((unsigned)blocks), norm_threads(s.tpr), 0, stream, a); e != cudaSuccess) return (int)e;
-    return (int)launch_early(kda_add_rms_norm_sum_kernel, dim3((a.D + 31) / 32), 1024, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)blocks);
+    return (int)(a.D <= 1024 ? launch_early(kda_add_rms_norm_sum_kernel<8>, dim3(a.D / 8), 1024, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)blocks)
+                             : launch_early(kda_add_rms_norm_sum_kernel<32>, dim3((a.D + 31) / 32), 1024, 0, stream, (const float*)a.part_w, a.dw, a.D, (int)blocks));
 }
 
 }  // namespace kda
