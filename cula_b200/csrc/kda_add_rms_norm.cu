@@ -433,11 +433,10 @@ __global__ void __launch_bounds__(1024) kda_add_rms_norm_sum_kernel(const float*
     if (lane == 0 && blockIdx.x * COLS + warp < D) dw[blockIdx.x * COLS + warp] = sum;
 }
 
-// Threads and pieces for a row: a warp up to 1024 columns, two pieces per thread above that. Where rows are few, one piece per thread
-// (forward): a row's latency is then the call's.
+// Threads and pieces for a row: as many threads as it has pieces, or pairs of pieces, in steps of some warps; idle threads cost loads that could
+// be on their way (2560 columns, backward, fp32 stream: 113 -> 101 us with 160 threads in the place of 256; 64 columns 182 -> 93 with 8 in
+// the place of 32). Where rows are few, one piece per thread (forward): a row's latency is then the call's.
 struct NormShape { int tpr, vpt; };
-// As many threads as a row has pieces, or pairs of pieces: idle ones cost loads that could be on their way (2560 columns, backward, fp32 stream:
-// 113 -> 101 us with 160 threads in the place of 256; 64 columns 182 -> 93 with 8 in the place of 32)
 static NormShape norm_shape(int D, long long R, bool backward) {
     const int nv = D / 8;
     if (nv <= 32) return {nv <= 8 ? 8 : nv <= 16 ? 16 : 32, 1};
@@ -486,7 +485,7 @@ static int launch_norm_bwd(const AddNormArgs& a, cudaStream_t stream) {
 
 }  // namespace kda
 
-// rows of `part_w` that the backward pass writes
+// rows of `part_w` that the backward pass writes at most
 extern "C" int kda_add_rms_norm_shares(int D, long long R) {
     using namespace kda;
     const NormShape s = norm_shape(D, R, true);
