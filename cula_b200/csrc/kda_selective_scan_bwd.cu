@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
                     for (int c = 0; c < 2; ++c) {
                         const float4 add = *reinterpret_cast<const float4*>(a.seg_state + (at + c) * SP + n0);
                         const float2 d = splat2(c ? sum.y : sum.x);
-                        gh[c][0] = fma2(ex2_2(mul2(d, A2[c][0])), gh[c][0], make_float2(add.x, add.y));
-                        gh[c][1] = fma2(ex2_2(mul2(d, A2[c][1])), gh[c][1], make_float2(add.z, add.w));
+                        gh[c][0] = fma2(decay2(d, A2[c][0]), gh[c][0], make_float2(add.x, add.y));
+                        gh[c][1] = fma2(decay2(d, A2[c][1]), gh[c][1], make_float2(add.z, add.w));
                     }
                 }
             }
@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const float2 d = splat2(c ? dx.y : dx.x), o = splat2(c ? dy.y : dy.x);
-                        gh[c][0] = mul2(ex2_2(mul2(d, A2[c][0])), fma2(o, make_float2(cc.x, cc.y), gh[c][0]));
-                        gh[c][1] = mul2(ex2_2(mul2(d, A2[c][1])), fma2(o, make_float2(cc.z, cc.w), gh[c][1]));
+                        gh[c][0] = mul2(decay2(d, A2[c][0]), fma2(o, make_float2(cc.x, cc.y), gh[c][0]));
+                        gh[c][1] = mul2(decay2(d, A2[c][1]), fma2(o, make_float2(cc.z, cc.w), gh[c][1]));
                     }
                 }
             } else {
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(SEL_BWD_THREADS, 2) kda_selective_scan_bwd_ker
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             const float2 d = splat2(c ? dx.y : dx.x), p = splat2(c ? dx.w : dx.z);
-                            av[u][c][0] = ex2_2(mul2(d, A2[c][0]));
-                            av[u][c][1] = ex2_2(mul2(d, A2[c][1]));
+                            av[u][c][0] = decay2(d, A2[c][0]);
+                            av[u][c][1] = decay2(d, A2[c][1]);
                             st[u + 1][c][0] = fma2(p, make_float2(b.x, b.y), mul2(av[u][c][0], st[u][c][0]));
                             st[u + 1][c][1] = fma2(p, make_float2(b.z, b.w), mul2(av[u][c][1], st[u][c][1]));
                         }

@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
                 for (int c = 0; c < 2; ++c) {
                     const float4 add = *reinterpret_cast<const float4*>(a.seg_state + (at + c) * SP + n0);
                     const float2 d = splat2(c ? sum.y : sum.x);
-                    h[c][0] = fma2(ex2_2(mul2(d, A2[c][0])), h[c][0], make_float2(add.x, add.y));
-                    h[c][1] = fma2(ex2_2(mul2(d, A2[c][1])), h[c][1], make_float2(add.z, add.w));
+                    h[c][0] = fma2(decay2(d, A2[c][0]), h[c][0], make_float2(add.x, add.y));
+                    h[c][1] = fma2(decay2(d, A2[c][1]), h[c][1], make_float2(add.z, add.w));
                 }
             }
         }
@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const float2 d = splat2(c ? dx.y : dx.x), p = splat2(c ? dx.w : dx.z);
-                h[c][0] = fma2(p, make_float2(b.x, b.y), mul2(ex2_2(mul2(d, A2[c][0])), h[c][0]));
-                h[c][1] = fma2(p, make_float2(b.z, b.w), mul2(ex2_2(mul2(d, A2[c][1])), h[c][1]));
+                h[c][0] = fma2(p, make_float2(b.x, b.y), mul2(decay2(d, A2[c][0]), h[c][0]));
+                h[c][1] = fma2(p, make_float2(b.z, b.w), mul2(decay2(d, A2[c][1]), h[c][1]));
                 if (!STATE_ONLY) {
                     const float2 q = fma2(make_float2(cc.z, cc.w), h[c][1], mul2(make_float2(cc.x, cc.y), h[c][0]));
                     v[2 * u + c] = q.x + q.y;

@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(STEP_THREADS, step_resident(SL)) kda_selective
                 B = step_four(static_cast<const T*>(a.Bm) + row * a.b_row + group * a.S, n0, a.S, a.vec);
                 C = step_four(static_cast<const T*>(a.Cm) + row * a.c_row + group * a.S, n0, a.S, a.vec);
             }
-            h.x = fmaf(fast_exp2(e * A[c].x), h.x, p * B.x);
-            h.y = fmaf(fast_exp2(e * A[c].y), h.y, p * B.y);
-            h.z = fmaf(fast_exp2(e * A[c].z), h.z, p * B.z);
-            h.w = fmaf(fast_exp2(e * A[c].w), h.w, p * B.w);
+            h.x = fmaf(decay(e, A[c].x), h.x, p * B.x);
+            h.y = fmaf(decay(e, A[c].y), h.y, p * B.y);
+            h.z = fmaf(decay(e, A[c].z), h.z, p * B.z);
+            h.w = fmaf(decay(e, A[c].w), h.w, p * B.w);
             v[c] = fmaf(h.x, C.x, h.y * C.y) + fmaf(h.z, C.z, h.w * C.w);
             if (d0 + c * CG + g < a.D) {
                 float* to = st + (size_t)d * a.S + n0;

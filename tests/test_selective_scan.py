@@ -227,6 +227,24 @@ def test_sequences_cut_into_segments(lens, T, D, S):
 
 
 @pytest.mark.gpu
+def test_errors_do_not_add_up_over_a_memory():
+    """Fast and slow channels in 32 bits. The exponential's mean error, at most 2^-26 where states remember up to 56 tokens, adds up to 8.4e-7;
+    three roundings per token, at most 2^-24 and independent, to 3^0.5 (2 x 56)^0.5 2^-25 in root mean square, there and back (5.5e-7): 1e-6
+    for both in quadrature, a quarter more for the spread between channels."""
+    from cula_b200.kda import selective_scan
+    a = make(2, 200, 64, 32, 1, torch.float32, h0=2, seed=21)
+    gen = torch.Generator().manual_seed(22)
+    dy, df = torch.randn(2, 200, 64, generator=gen), 0.1 * torch.randn(2, 64, 32, generator=gen)
+    leaves = [k for k, v in a.items() if torch.is_tensor(v)]
+    r, d = in64(a, True), on_gpu(a, True)
+    ref, got = selective_scan_ref(**r), selective_scan(**d, output_final_state=True)
+    g_ref = torch.autograd.grad(ref, [r[k] for k in leaves], [dy.double(), df.double()])
+    g_got = torch.autograd.grad(got, [d[k] for k in leaves], [dy.cuda(), df.cuda()])
+    errors = {k: err_ratio(u.detach(), v.detach().double().cpu()) for k, u, v in zip(["y", "fin"] + leaves, [*ref, *g_ref], [*got, *g_got])}
+    assert all(e < 1.25e-6 for e in errors.values()), errors
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from cula_b200.kda import selective_scan
     a = on_gpu(make(2, 0, 16, 4, h0=2))
