@@ -490,9 +490,9 @@ inline int checked(int rc) { return rc == -1 ? CULA_KDA_EINVAL : rc; }
 int scan_args_error(const kda::SelScanArgs* a) {
     if (!a || !a->x || !a->dt || !a->Bm || !a->Cm || !a->A || a->D <= 0 || a->G <= 0 || a->S <= 0 || a->S > 64) return CULA_KDA_EINVAL;
     if (a->D % a->G || a->D / a->G % 8 || a->rows < 0 || a->n_seqs < 0 || a->num_chunks < 0 || a->seg_chunks < 0) return CULA_KDA_EINVAL;
+    // members that a call does not use may hold anything
     const bool packed = a->cu_seqlens != nullptr;
-    if (packed != (a->chunk_indices != nullptr) || packed != (a->chunk_offsets != nullptr) || packed != (a->seq_order != nullptr)) return CULA_KDA_EINVAL;
-    if (packed && (a->total_tokens < 0 || a->total_tokens > a->rows)) return CULA_KDA_EINVAL;
+    if (packed && (!a->chunk_offsets || (!a->seg_chunks && !a->seq_order) || a->total_tokens < 0 || a->total_tokens > a->rows)) return CULA_KDA_EINVAL;
     if (!packed && (a->T < 0 || a->rows != (long long)a->n_seqs * a->T || a->num_chunks != (long long)a->n_seqs * ((a->T + kda::BT - 1) / kda::BT)))
         return CULA_KDA_EINVAL;
     if (a->seg_chunks && (!a->seg_state || !a->seg_dt)) return CULA_KDA_EINVAL;
@@ -500,13 +500,14 @@ int scan_args_error(const kda::SelScanArgs* a) {
         if (row < 0 || row > 0x7fffffffLL) return CULA_KDA_EINVAL;
     const uintptr_t quad = a->fp32 ? 15 : 7;
     if (a->vec_bc && ((a->S % 4 && a->G > 1) || ((reinterpret_cast<uintptr_t>(a->Bm) | reinterpret_cast<uintptr_t>(a->Cm)) & quad) || a->b_row % 4 ||
-                      a->c_row % 4 || a->b_seq % 4 || a->c_seq % 4))
+                      a->c_row % 4 || (!packed && (a->b_seq % 4 || a->c_seq % 4))))
         return CULA_KDA_EALIGN;
     const int per = a->fp32 ? 4 : 8;
-    if (misaligned(a->x) || misaligned(a->dt) || misaligned(a->z) || a->x_row % per || a->dt_row % per || a->x_seq % per || a->dt_seq % per ||
-        (a->z && (a->z_row % per || a->z_seq % per)) || misaligned(a->states) || misaligned(a->seg_state) || misaligned(a->seg_dt) || misaligned(a->y_pre))
+    if (misaligned(a->x) || misaligned(a->dt) || misaligned(a->z) || a->x_row % per || a->dt_row % per || (a->z && a->z_row % per) || misaligned(a->states))
         return CULA_KDA_EALIGN;
-    return 0;
+    if (!packed && (a->x_seq % per || a->dt_seq % per || (a->z && a->z_seq % per))) return CULA_KDA_EALIGN;
+    if (a->seg_chunks && (misaligned(a->seg_state) || misaligned(a->seg_dt))) return CULA_KDA_EALIGN;
+    return a->z && a->states && misaligned(a->y_pre) ? CULA_KDA_EALIGN : 0;
 }
 }
 
@@ -525,7 +526,9 @@ extern "C" int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* a
     if (!a->y && a->rows) return CULA_KDA_EINVAL;
     if (a->z && a->states && !a->y_pre && a->rows) return CULA_KDA_EINVAL;
     if (misaligned(a->y)) return CULA_KDA_EALIGN;
-    return checked(kda_launch_selective_scan_fwd(a, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
+    kda::SelScanArgs used = *a;
+    if (!a->states) used.y_pre = nullptr;                            // the kernel writes where it is given a place
+    return checked(kda_launch_selective_scan_fwd(&used, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int cula_kda_selective_scan_bwd(const cula_kda_selective_scan_args* a, void* stream) {
@@ -533,10 +536,13 @@ extern "C" int cula_kda_selective_scan_bwd(const cula_kda_selective_scan_args* a
     if (a->rows == 0 || a->n_seqs == 0 || a->cta_rows <= 0 || !a->dy || !a->dx || !a->ddt || !a->dBm || !a->dCm || !a->dA || !a->part_bc || !a->part_A ||
         !a->states || (a->z && (!a->dz || !a->y_pre)) || (a->dskip && !a->part_skip) || (a->dbias && !a->part_bias))
         return CULA_KDA_EINVAL;
-    if (misaligned(a->dy) || misaligned(a->dx) || misaligned(a->ddt) || misaligned(a->dz) || misaligned(a->part_bc) || misaligned(a->part_A) ||
-        misaligned(a->part_skip) || misaligned(a->part_bias) || misaligned(a->skip) || misaligned(a->dt_bias))
+    if (misaligned(a->dy) || misaligned(a->dx) || misaligned(a->ddt) || (a->z && misaligned(a->dz)) || misaligned(a->part_bc) || misaligned(a->part_A) ||
+        (a->dskip && misaligned(a->part_skip)) || (a->dbias && misaligned(a->part_bias)))
         return CULA_KDA_EALIGN;
-    return checked(kda_launch_selective_scan_bwd(a, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
+    kda::SelScanArgs used = *a;
+    if (!a->dskip) used.part_skip = nullptr;
+    if (!a->dbias) used.part_bias = nullptr;
+    return checked(kda_launch_selective_scan_bwd(&used, state_lanes(a->S), static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int cula_kda_selective_step(const cula_kda_selective_step_args* a, void* stream) {
@@ -573,8 +579,8 @@ extern "C" int cula_kda_add_rms_norm_fwd(const cula_kda_add_rms_norm_args* a, vo
     if (a->R == 0) return 0;
     if (!a->x || !a->w || !a->y || (a->res && (!a->r || !a->r_out)) || (a->fp8 && !a->scale)) return CULA_KDA_EINVAL;
     if (a->fp8 && a->group && ((a->group != 32 && a->group != 64 && a->group != 128 && a->group != 256) || a->D % a->group)) return CULA_KDA_EINVAL;
-    if (misaligned(a->x) || misaligned(a->r) || misaligned(a->w) || misaligned(a->y) || misaligned(a->r_out) || a->x_row % (a->fp32 ? 4 : 8) ||
-        (a->res && a->r_row % (a->res == 2 ? 4 : 8)))
+    if (misaligned(a->x) || misaligned(a->w) || misaligned(a->y) || a->x_row % (a->fp32 ? 4 : 8) ||
+        (a->res && (misaligned(a->r) || misaligned(a->r_out) || a->r_row % (a->res == 2 ? 4 : 8))))
         return CULA_KDA_EALIGN;
     return checked(kda_launch_add_rms_norm(a, 0, static_cast<cudaStream_t>(stream)));
 }
@@ -582,8 +588,8 @@ extern "C" int cula_kda_add_rms_norm_fwd(const cula_kda_add_rms_norm_args* a, vo
 extern "C" int cula_kda_add_rms_norm_bwd(const cula_kda_add_rms_norm_args* a, void* stream) {
     if (const int e = norm_args_error(a)) return e;
     if (a->R == 0 || !a->v || !a->w || !a->rstd || !a->dy || !a->dx || !a->part_w || !a->dw) return CULA_KDA_EINVAL;
-    if (misaligned(a->v) || misaligned(a->w) || misaligned(a->dy) || misaligned(a->dr_out) || misaligned(a->dx) || misaligned(a->dr) || misaligned(a->part_w) ||
-        (!a->res && a->x_row % (a->fp32 ? 4 : 8)))
+    if (misaligned(a->v) || misaligned(a->w) || misaligned(a->dy) || misaligned(a->dx) || misaligned(a->part_w) ||
+        (a->res && (misaligned(a->dr_out) || misaligned(a->dr))) || (!a->res && a->x_row % (a->fp32 ? 4 : 8)))
         return CULA_KDA_EALIGN;
     return checked(kda_launch_add_rms_norm(a, 1, static_cast<cudaStream_t>(stream)));
 }

@@ -343,7 +343,8 @@ typedef struct cula_kda_selective_scan_args {
     float *part_skip, *part_bias;
     float* seg_state;             /* with seg_chunks, workspaces [segments, D, SP] and [segments, D]; segments = N ceil(chunks / seg_chunks), */
     float* seg_dt;                /* or num_chunks / seg_chunks + N for a packed batch */
-    const int *cu_seqlens, *chunk_indices, *chunk_offsets, *seq_order;      /* packed batch (cula_kda_build_chunk_tables), or NULL */
+    const int *cu_seqlens, *chunk_indices, *chunk_offsets, *seq_order;      /* packed batch (cula_kda_build_chunk_tables), or cu_seqlens NULL;
+                                     chunk_indices is not used, nor seq_order with seg_chunks */
     long long rows;               /* B*T */
     int T, D, S, G, n_seqs, num_chunks, total_tokens;       /* total_tokens: of a packed batch */
     int seg_chunks;               /* 0: sequences are not cut */

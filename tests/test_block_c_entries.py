@@ -1,0 +1,78 @@
+"""The C entries of a state space block's operators: what they refuse, and that members which a call does not use may hold anything. On
+the CPU an accepted call ends with the runtime's error (there is no device, so that nothing is launched), which is above zero."""
+import pytest
+import torch
+
+from tests.block_c import GARBAGE, ConvStepArgs, NormArgs, ScanArgs, StepArgs, call
+
+EINVAL, EALIGN = -1, -2
+AT = 0x10000                                                         # aligned; never read, since nothing is launched without a device
+cpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are made up: only without a device")
+
+
+def scan(**change):
+    """A scan of two sequences of 70 tokens, 16 channels, 4 states, without anything optional."""
+    a = dict(x=AT, dt=AT, Bm=AT, Cm=AT, A=AT, y=AT, x_row=16, dt_row=16, b_row=4, c_row=4, x_seq=16 * 70, dt_seq=16 * 70, b_seq=4 * 70, c_seq=4 * 70,
+             rows=140, T=70, D=16, S=4, G=1, n_seqs=2, num_chunks=4, states=AT, dy=AT, dx=AT, ddt=AT, dBm=AT, dCm=AT, dA=AT, part_bc=AT, part_A=AT,
+             cta_rows=1, vec_bc=1)
+    return ScanArgs(**{**a, **change})
+
+
+def packed(**change):
+    return scan(**{**dict(cu_seqlens=AT, chunk_offsets=AT, seq_order=AT, total_tokens=140, x_seq=0, dt_seq=0, b_seq=0, c_seq=0), **change})
+
+
+def norm(**change):
+    a = dict(x=AT, w=AT, y=AT, v=AT, rstd=AT, dy=AT, dx=AT, part_w=AT, dw=AT, R=3, x_row=64, D=64, eps=1e-6)
+    return NormArgs(**{**a, **change})
+
+
+@cpu_only
+@pytest.mark.parametrize("entry", ["selective_scan_fwd", "selective_scan_bwd"])
+def test_members_that_a_scan_does_not_use_may_hold_anything(entry):
+    assert call(entry, scan()) > 0 and call(entry, packed()) > 0
+    for members in ("seg_state seg_dt", "z_row z_seq y_pre dz", "part_skip part_bias", "chunk_indices", "chunk_offsets seq_order", "total_tokens"):
+        assert call(entry, scan(**{m: GARBAGE for m in members.split()})) > 0, members
+    for members in ("chunk_indices", "x_seq dt_seq z_seq b_seq c_seq", "T", "seg_state seg_dt"):
+        assert call(entry, packed(**{m: GARBAGE for m in members.split()})) > 0, members
+    assert call(entry, packed(seg_chunks=1, seg_state=AT, seg_dt=AT, seq_order=None)) > 0
+    # what a call does use is looked at as before
+    assert call(entry, scan(seg_chunks=1, seg_state=GARBAGE, seg_dt=AT)) == EALIGN and call(entry, scan(seg_chunks=1)) == EINVAL
+    assert call(entry, scan(x_seq=3)) == EALIGN and call(entry, scan(z=AT, z_row=3, y_pre=AT, dz=AT)) == EALIGN
+    assert call(entry, scan(z=AT, z_row=16, z_seq=1120, y_pre=GARBAGE, dz=AT)) == EALIGN
+    assert call(entry, packed(chunk_offsets=None)) == EINVAL and call(entry, packed(seq_order=None)) == EINVAL
+    if entry.endswith("bwd"):
+        assert call(entry, scan(dz=GARBAGE, z=AT, z_row=16, z_seq=1120, y_pre=AT)) == EALIGN
+        assert call(entry, scan(dskip=AT)) == EINVAL and call(entry, scan(dskip=AT, part_skip=GARBAGE)) == EALIGN
+        assert call(entry, scan(skip=AT + 4, dt_bias=AT + 4)) > 0    # read one by one, as in the forward pass
+
+
+@cpu_only
+def test_members_that_a_norm_does_not_use_may_hold_anything():
+    for entry, members in (("add_rms_norm_fwd", "r r_out r_row scale v dy dr_out dx dr part_w dw"), ("add_rms_norm_bwd", "dr_out dr r r_out r_row x y scale")):
+        assert call(entry, norm(**{m: GARBAGE for m in members.split()})) > 0
+    assert call("add_rms_norm_fwd", norm(res=1, r=GARBAGE, r_out=AT, r_row=64)) == EALIGN
+    assert call("add_rms_norm_bwd", norm(res=1, dr_out=GARBAGE)) == EALIGN
+
+
+@pytest.mark.gpu
+def test_workspaces_that_a_scan_does_not_use_are_not_written():
+    """y before the gate is kept with the states only, and shares of dskip and dbias are written where these gradients are asked for."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    rn = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    T, D, S = 20, 16, 4
+    x, dt, z, dy, Bm, Cm, A = rn(T, D), rn(T, D).abs(), rn(T, D), rn(T, D), rn(T, S), rn(T, S), -rn(D, S).abs()
+    out = {k: torch.empty(T, D, device="cuda") for k in ("y", "dx", "ddt", "dz")}
+    bc = {k: torch.empty(T, S, device="cuda") for k in ("dBm", "dCm")}
+    spare = torch.full((T, D), 7.0, device="cuda")
+    own = dict(states=torch.empty(8 * 1024, device="cuda"), y_pre=torch.empty(T, D, device="cuda"), dA=torch.empty(D, S, device="cuda"),
+               part_bc=torch.empty(T * 16, device="cuda"), part_A=torch.empty(D * 8, device="cuda"))
+    at = lambda ts: {k: t.data_ptr() for k, t in ts.items()}  # noqa: E731
+    base = dict(x=x.data_ptr(), dt=dt.data_ptr(), z=z.data_ptr(), Bm=Bm.data_ptr(), Cm=Cm.data_ptr(), A=A.data_ptr(), x_row=D, dt_row=D, z_row=D, b_row=S, c_row=S,
+                rows=T, T=T, D=D, S=S, G=1, n_seqs=1, num_chunks=1, fp32=1, cta_rows=1, dy=dy.data_ptr(), **at(out), **at(bc))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert call("selective_scan_fwd", ScanArgs(**base, y_pre=spare.data_ptr()), stream) == 0
+    assert call("selective_scan_fwd", ScanArgs(**base, **at({k: own[k] for k in ("states", "y_pre")})), stream) == 0
+    assert call("selective_scan_bwd", ScanArgs(**base, **at(own), part_skip=spare.data_ptr(), part_bias=spare.data_ptr()), stream) == 0
+    torch.cuda.synchronize()
+    assert (spare == 7.0).all() and own["dA"].isfinite().all()
