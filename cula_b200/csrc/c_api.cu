@@ -487,11 +487,15 @@ extern "C" int kda_add_rms_norm_shares(int D, long long R);
 namespace {
 inline int state_lanes(int S) { return S <= 8 ? 2 : S <= 16 ? 4 : S <= 32 ? 8 : 16; }
 inline int checked(int rc) { return rc == -1 ? CULA_KDA_EINVAL : rc; }
+// What the kernels count in 32 bits, some way past the end among it: tokens of a sequence, rows of a step, channels, and chunks of a segment
+// (times 64, behind a token)
+constexpr int MOST_TOKENS = 1 << 30, MOST_CHANNELS = 1 << 24, MOST_SEG_CHUNKS = MOST_TOKENS / kda::BT;
 int scan_args_error(const kda::SelScanArgs* a) {
     if (!a || !a->x || !a->dt || !a->Bm || !a->Cm || !a->A || a->D <= 0 || a->G <= 0 || a->S <= 0 || a->S > 64) return CULA_KDA_EINVAL;
     if (a->D % a->G || a->D / a->G % 8 || a->rows < 0 || a->n_seqs < 0 || a->num_chunks < 0 || a->seg_chunks < 0) return CULA_KDA_EINVAL;
     // members that a call does not use may hold anything
     const bool packed = a->cu_seqlens != nullptr;
+    if (a->D > MOST_CHANNELS || (packed ? a->total_tokens : a->T) > MOST_TOKENS || a->seg_chunks > MOST_SEG_CHUNKS) return CULA_KDA_EINVAL;
     if (packed && (!a->chunk_offsets || (!a->seg_chunks && !a->seq_order) || a->total_tokens < 0 || a->total_tokens > a->rows)) return CULA_KDA_EINVAL;
     if (!packed && (a->T < 0 || a->rows != (long long)a->n_seqs * a->T || a->num_chunks != (long long)a->n_seqs * ((a->T + kda::BT - 1) / kda::BT)))
         return CULA_KDA_EINVAL;
@@ -550,7 +554,7 @@ extern "C" int cula_kda_selective_step(const cula_kda_selective_step_args* a, vo
     if (a->rows == 0) return 0;
     if (!a->x || !a->dt || !a->Bm || !a->Cm || !a->A || !a->state || !a->y || !a->status || a->D <= 0 || a->G <= 0 || a->D % a->G || a->S <= 0 || a->S > 64)
         return CULA_KDA_EINVAL;
-    if (!a->indices && a->pool < a->rows) return CULA_KDA_EINVAL;
+    if (a->rows > MOST_TOKENS || a->D > MOST_CHANNELS || (!a->indices && a->pool < a->rows)) return CULA_KDA_EINVAL;
     const uintptr_t quad = a->fp32 ? 15 : 7;
     if (a->vec && (a->S % 4 || misaligned(a->state) || misaligned(a->A) || a->b_row % 4 || a->c_row % 4 ||
                    ((reinterpret_cast<uintptr_t>(a->Bm) | reinterpret_cast<uintptr_t>(a->Cm)) & quad)))
@@ -562,7 +566,7 @@ extern "C" int cula_kda_conv_step(const cula_kda_conv_step_args* a, void* stream
     if (!a || a->rows < 0) return CULA_KDA_EINVAL;
     if (a->rows == 0) return 0;
     if (!a->x || !a->w || !a->cache || !a->y || !a->status || a->D <= 0 || a->D % 8 || a->W < 1 || a->W > 4) return CULA_KDA_EINVAL;
-    if (!a->indices && a->pool < a->rows) return CULA_KDA_EINVAL;
+    if (a->rows > MOST_TOKENS || a->D > MOST_CHANNELS || (!a->indices && a->pool < a->rows)) return CULA_KDA_EINVAL;
     if (misaligned(a->w) || misaligned(a->cache) || misaligned(a->y) || (reinterpret_cast<uintptr_t>(a->x) & 3) || a->x_row % 2) return CULA_KDA_EALIGN;
     return checked(kda_launch_conv_step(a, static_cast<cudaStream_t>(stream)));
 }

@@ -315,7 +315,8 @@ int cula_kda_rms_norm_gated_bwd(const void* d_x, const void* d_g, const float* d
  * Rows of x, dt, z, B and C may be strided (row: elements from a token to the next, seq: from a sequence of a fixed-length batch to the
  * next; row strides fit 31 bits); their innermost dimensions are contiguous, rows of x, dt and z are 16-byte aligned, D / G is a multiple of 8, S <= 64. Everything
  * else is contiguous. A sequence is walked in one piece, or (seg_chunks) in segments of that many 64-token chunks side by side, for which a
- * launch before finds what each adds to the state.
+ * launch before finds what each adds to the state. At most 2^30 tokens per sequence (or packed batch), or rows per step, 2^24 channels and
+ * 2^24 chunks per segment.
  * SP below is the smallest of 8, 16, 32 and 64 that holds S.
  * ------------------------------------------------------------------------------------------------------------ */
 typedef struct cula_kda_selective_scan_args {

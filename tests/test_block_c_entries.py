@@ -55,6 +55,26 @@ def test_members_that_a_norm_does_not_use_may_hold_anything():
     assert call("add_rms_norm_bwd", norm(res=1, dr_out=GARBAGE)) == EALIGN
 
 
+@cpu_only
+def test_sizes_at_which_counts_would_pass_32_bits_are_refused():
+    most = 2 ** 30
+    for entry in ("selective_scan_fwd", "selective_scan_bwd"):
+        seg = dict(seg_state=AT, seg_dt=AT)
+        assert call(entry, scan(seg_chunks=2 ** 24, **seg)) > 0      # one segment each; 2^26 chunks of 64 tokens are 0 in 32 bits
+        for chunks in (2 ** 24 + 1, 2 ** 25, 2 ** 26, 2 ** 31 - 1):
+            assert call(entry, scan(seg_chunks=chunks, **seg)) == EINVAL and call(entry, packed(seg_chunks=chunks, **seg)) == EINVAL
+        assert call(entry, scan(T=most + 1, n_seqs=1, rows=most + 1, num_chunks=2 ** 24 + 1)) == EINVAL
+        assert call(entry, packed(total_tokens=most + 1, rows=most + 1)) == EINVAL
+        assert call(entry, scan(D=2 ** 24 + 8, x_row=2 ** 24 + 8, dt_row=2 ** 24 + 8)) == EINVAL
+    step = dict(x=AT, dt=AT, Bm=AT, Cm=AT, A=AT, state=AT, y=AT, indices=AT, status=AT, D=16, S=4, G=1, pool=1, x_row=16, dt_row=16, b_row=4, c_row=4)
+    conv = dict(x=AT, w=AT, cache=AT, y=AT, indices=AT, status=AT, D=16, W=4, pool=1, x_row=16)
+    for entry, args, kind in (("selective_step", step, StepArgs), ("conv_step", conv, ConvStepArgs)):
+        assert call(entry, kind(**args, rows=most)) > 0
+        for rows in (most + 1, 2 ** 31 - 1):                         # rows ahead of the last one are numbered too
+            assert call(entry, kind(**args, rows=rows)) == EINVAL
+        assert call(entry, kind(**{**args, "D": 2 ** 24 + 8}, rows=1)) == EINVAL
+
+
 @pytest.mark.gpu
 def test_workspaces_that_a_scan_does_not_use_are_not_written():
     """y before the gate is kept with the states only, and shares of dskip and dbias are written where these gradients are asked for."""
