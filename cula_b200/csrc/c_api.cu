@@ -521,7 +521,8 @@ extern "C" int cula_kda_selective_scan_tiles(int D, int G, int S) {
 
 extern "C" int cula_kda_selective_scan_state_floats(int D, int G, int S) {
     const int tiles = cula_kda_selective_scan_tiles(D, G, S);
-    return tiles < 0 ? tiles : tiles * G * 1024;                     // 128 threads of a tile hold 8 each
+    const long long floats = (long long)tiles * G * 1024;            // 128 threads of a tile hold 8 each
+    return tiles < 0 || floats > 0x7fffffffLL ? CULA_KDA_EINVAL : (int)floats;
 }
 
 extern "C" int cula_kda_selective_scan_fwd(const cula_kda_selective_scan_args* a, void* stream) {

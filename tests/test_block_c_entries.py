@@ -75,6 +75,14 @@ def test_sizes_at_which_counts_would_pass_32_bits_are_refused():
         assert call(entry, kind(**{**args, "D": 2 ** 24 + 8}, rows=1)) == EINVAL
 
 
+def test_kept_states_that_an_int_cannot_count_are_refused():
+    from cula_b200 import _native
+    floats = _native.lib().cula_kda_selective_scan_state_floats
+    assert floats(2 ** 23, 2 ** 20, 16) == 2 ** 30                   # a tile of 1024 per group
+    for D, G in ((2 ** 24, 2 ** 21), (2 ** 24, 2 ** 22)):
+        assert floats(D, G, 16) == EINVAL
+
+
 @pytest.mark.gpu
 def test_workspaces_that_a_scan_does_not_use_are_not_written():
     """y before the gate is kept with the states only, and shares of dskip and dbias are written where these gradients are asked for."""
