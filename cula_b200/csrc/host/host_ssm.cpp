@@ -27,6 +27,13 @@ bool grad_wanted(std::initializer_list<OptTensor> ts) {
         if (t.has_value() && t->defined() && t->requires_grad()) return true;
     return false;
 }
+// an operator without gradients: a tangent would be lost without a word
+using cula_host::has_tangent;
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... Ts>
+void refuse_tangents(const char* op, const Ts&... ts) {
+    if ((has_tangent(ts) || ...)) throw std::runtime_error(std::string(op) + " has no forward derivative");
+}
 OptTensor opt_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 bool is_float(const Tensor& t) { return is_bf16(t) || is_f32(t); }
@@ -370,6 +377,7 @@ Tensor output_of(const OptTensor& out, const Tensor& x) { return has(out) ? *out
 Tensor selective_scan_update(const Tensor& x_in, const Tensor& dt_in, const Tensor& A_in, const Tensor& B_in, const Tensor& C_in, const Tensor& state,
                              const OptTensor& indices, const OptTensor& skip_in, const OptTensor& z_in, const OptTensor& bias_in, bool softplus,
                              const OptTensor& out_in) {
+    refuse_tangents("selective_scan_update", x_in, dt_in, A_in, B_in, C_in, state, skip_in, z_in, bias_in);
     at::NoGradGuard no_grad;
     const bool with_time = x_in.dim() == 3;
     require(x_in.dim() == 2 || (with_time && x_in.size(1) == 1), "x must be [N, D] or [N, 1, D].");
@@ -410,6 +418,7 @@ Tensor selective_scan_update(const Tensor& x_in, const Tensor& dt_in, const Tens
 
 Tensor short_conv_update(const Tensor& x_in, const Tensor& weight_in, const Tensor& cache, const OptTensor& indices, const OptTensor& bias_in, bool silu,
                          const OptTensor& out_in) {
+    refuse_tangents("short_conv_update", x_in, weight_in, cache, bias_in);
     at::NoGradGuard no_grad;
     const bool with_time = x_in.dim() == 3;
     require((x_in.dim() == 2 || (with_time && x_in.size(1) == 1)) && is_bf16(x_in), "x must be [N, D] or [N, 1, D] in bfloat16.");
@@ -542,6 +551,7 @@ std::pair<Tensor, OptTensor> add_rms_norm(const Tensor& x, const Tensor& weight,
     return {o.y, opt_of(o.r_out)};
 }
 std::tuple<Tensor, Tensor, OptTensor> add_rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& r, double eps, int64_t group) {
+    refuse_tangents("add_rms_norm_fp8", x, weight, r);
     if (group) {
         require(group == 32 || group == 64 || group == 128 || group == 256, "group_size must be 32, 64, 128, 256 or None.");
         require(x.dim() >= 1 && x.size(-1) % group == 0, "the normalised dim must be a multiple of group_size.");

@@ -70,6 +70,21 @@ def test_refusals():
             short_conv_update(x, cw, cache)
 
 
+def test_tangents_are_refused_not_dropped():
+    """The operators without gradients have no forward derivatives either."""
+    import torch.autograd.forward_ad as fw
+
+    from cula_b200.kda import add_rms_norm_fp8, selective_scan_update, short_conv_update
+    x, A, bc, one = torch.ones(2, 16).bfloat16(), -torch.ones(16, 4), torch.ones(2, 4).bfloat16(), torch.ones(16)
+    calls = [(selective_scan_update, dict(x=x, dt=x, A=A, B=bc, C=bc, state=torch.zeros(2, 16, 4), D=one, z=x, dt_bias=one)),
+             (short_conv_update, dict(x=x, weight=torch.ones(16, 4), cache=torch.zeros(2, 16, 4), bias=one)),
+             (add_rms_norm_fp8, dict(x=x, weight=one, residual=x))]
+    for call, args in calls:
+        for name in args:
+            with fw.dual_level(), pytest.raises(RuntimeError, match="no forward derivative"):
+                call(**{**args, name: fw.make_dual(args[name], torch.ones_like(args[name]))})
+
+
 # ------------------------------------------------ residual RMS norm ------------------------------------------------
 NORMS = [(1, 8, "bf16", "bf16"), (5, 64, "fp32", "fp32"), (3, 264, "bf16", "fp32"), (33, 520, "bf16", "none"), (7, 1000, "fp32", "none"), (333, 1024, "bf16", "bf16"),
          (2, 1032, "bf16", "bf16"), (400, 2056, "bf16", "fp32"), (5, 4096, "bf16", "bf16"), (310, 4096, "fp32", "fp32"), (9, 4104, "bf16", "none"), (6, 8192, "fp32", "fp32"),
