@@ -176,9 +176,7 @@ __global__ void __launch_bounds__(SEL_FWD_THREADS, 2) kda_selective_scan_fwd_ker
     for (int c = 0; c < 2; ++c) {
         h[c][0] = h[c][1] = A2[c][0] = A2[c][1] = make_float2(0.f, 0.f);
         if (own) {
-            sel_load4(a.A + (size_t)(dc + c) * a.S, n0, a.S, A2[c]);
-            A2[c][0] = mul2(A2[c][0], splat2(RCP_LN2));
-            A2[c][1] = mul2(A2[c][1], splat2(RCP_LN2));
+            sel_load_rates(a.A + (size_t)(dc + c) * a.S, n0, a.S, A2[c]);
             if (!STATE_ONLY && a.h0) sel_load4(a.h0 + ((size_t)it.seq * a.D + dc + c) * a.S, n0, a.S, h[c]);
         }
     }

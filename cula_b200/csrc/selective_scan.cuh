@@ -9,6 +9,8 @@
 // neighbouring lanes ask for the same address takes 2.3 cycles of the SM instead of 4. Lane cl of warp w has channels 8 cl + 2 w and the
 // next: what one thread stages, a piece of 8 channels, is a pair for each warp, and both sides touch shared memory in order.
 #pragma once
+#include <cfloat>
+
 #include "kda_common.cuh"
 #include "kda_params.h"
 
@@ -140,6 +142,17 @@ __device__ __forceinline__ void sel_load4(const float* row, int n, int S, float2
     float f[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) f[k] = n + k < S ? row[n + k] : 0.f;
+    v[0] = make_float2(f[0], f[1]); v[1] = make_float2(f[2], f[3]);
+}
+// four rates, for exponents of two. One of minus infinity is held as the lowest number: tokens past the end of a tile have steps of zero, which
+// change no state, while zero times infinity would
+__device__ __forceinline__ void sel_load_rates(const float* row, int n, int S, float2 (&v)[2]) {
+    float f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float r = n + k < S ? row[n + k] * RCP_LN2 : 0.f;
+        f[k] = r == -INFINITY ? -FLT_MAX : r;
+    }
     v[0] = make_float2(f[0], f[1]); v[1] = make_float2(f[2], f[3]);
 }
 __device__ __forceinline__ void sel_store4(float* row, int n, int S, const float2 (&v)[2]) {

@@ -245,6 +245,26 @@ def test_errors_do_not_add_up_over_a_memory():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [13, 16, 75])
+def test_states_that_forget_at_once(T):
+    """Rates of minus infinity: such a state holds its token alone. The last tile of tokens is whole or not."""
+    from cula_b200.kda import selective_scan
+    a = make(2, T, 24, 6, 1, torch.float32, h0=2, seed=T)
+    a["A"][::2, 1::2] = float("-inf")
+    gen = torch.Generator().manual_seed(23)
+    dy, df = torch.randn(2, T, 24, generator=gen), torch.randn(2, 24, 6, generator=gen)
+    leaves = ["x", "A", "B", "C", "D", "z", "initial_state"]         # of dt, autograd's derivative of the oracle is 0 times infinity
+    r, d = in64(a, True), on_gpu(a, True)
+    ref, got = selective_scan_ref(**r), selective_scan(**d, output_final_state=True)
+    assert got[1].isfinite().all()
+    g_ref = torch.autograd.grad(ref, [r[k] for k in leaves], [dy.double(), df.double()])
+    g_got = torch.autograd.grad(got, [d[k] for k in leaves + ["dt"]], [dy.cuda(), df.cuda()])
+    for k, u, v in zip(["y", "fin"] + leaves, [*ref, *g_ref], [*got, *g_got]):
+        assert err_ratio(u.detach(), v.detach().double().cpu()) < tol(torch.float32, T), k
+    assert g_got[-1].isfinite().all()
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     from cula_b200.kda import selective_scan
     a = on_gpu(make(2, 0, 16, 4, h0=2))
