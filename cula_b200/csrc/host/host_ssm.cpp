@@ -372,6 +372,10 @@ void check_out(const OptTensor& out, const Tensor& x) {
         throw pybind11::value_error("out must be a contiguous, 16-byte aligned tensor of the shape and type of x");
     on_device_of(x, {{out, "out"}});
 }
+// autograd learns that a tensor was written to: a graph that has kept it must not take it for what it was
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Tensor output_of(const OptTensor& out, const Tensor& x) { return has(out) ? *out : device_empty(x.sizes(), x.options()); }
 
 Tensor selective_scan_update(const Tensor& x_in, const Tensor& dt_in, const Tensor& A_in, const Tensor& B_in, const Tensor& C_in, const Tensor& state,
@@ -413,6 +417,8 @@ Tensor selective_scan_update(const Tensor& x_in, const Tensor& dt_in, const Tens
     a.vec = S % 4 == 0 && a.b_row % 4 == 0 && a.c_row % 4 == 0 && aligned(Br, quad) && aligned(Cr, quad) && aligned(state);
     a.status = status_word(x.device().index());
     check(lib.cula_kda_selective_step(&a, stream_of(x)), "cula_kda_selective_step");
+    written(state);
+    if (has(out_in)) written(out);
     return out;
 }
 
@@ -447,6 +453,8 @@ Tensor short_conv_update(const Tensor& x_in, const Tensor& weight_in, const Tens
     a.rows = (int)N; a.D = (int)D; a.W = (int)W; a.pool = (int)cache.size(0); a.silu = silu;
     a.status = status_word(x.device().index());
     check(lib.cula_kda_conv_step(&a, stream_of(x)), "cula_kda_conv_step");
+    written(cache);
+    if (has(out_in)) written(out);
     return out;
 }
 

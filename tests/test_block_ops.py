@@ -333,6 +333,24 @@ def test_conv_step_continues_a_prompt_bit_for_bit():
         check_status(torch.device("cuda", 0))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["state", "out"])
+def test_what_a_step_changes_in_place_is_not_taken_for_unchanged(which):
+    """A graph that has kept a pool, or the place of an output, for its backward pass says so when a step has written to it since."""
+    from cula_b200.kda import selective_scan_update, short_conv_update
+    x, A, bc = torch.ones(2, 16, device="cuda").bfloat16(), -torch.ones(16, 4, device="cuda"), torch.ones(2, 4, device="cuda").bfloat16()
+    for step in (lambda pool, out: selective_scan_update(x, x, A, bc, bc, pool, out=out), lambda pool, out: short_conv_update(x, -A, pool, out=out)):
+        pool, out = (torch.ones(2, 16, 4, device="cuda", requires_grad=True) * 2), (torch.ones(2, 16, device="cuda").bfloat16().requires_grad_(True) * 2)
+        loss = (pool if which == "state" else out).square().sum()
+        step(pool.detach() if which == "out" else pool, out if which == "out" else None)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        pool = torch.ones(2, 16, 4, device="cuda")
+    step(pool, None)                                                 # has no version: nothing to tell, nothing refused
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------ a whole block ------------------------------------------------
 def block(p, x, res, ops):
     """norm -> input projection -> convolution -> projections to step, B and C -> scan, gated -> output projection; returns (out, stream)."""
