@@ -574,6 +574,12 @@ std::tuple<Tensor, Tensor, OptTensor> add_rms_norm_fp8(const Tensor& x, const Te
 
 void bind_ssm(pybind11::module_& m) {
     m.def("selective_scan", &selective_scan);
+    // the planner alone: chunks per segment for so many sequences and chunks, the longest sequence's, and tiles of channels; 0: not cut
+    m.def("selective_scan_segments", [](int64_t n_seqs, int64_t num_chunks, int64_t longest, int64_t tiles, bool packed, bool backward) {
+        ScanSizes s{};
+        s.n_seqs = n_seqs; s.num_chunks = num_chunks; s.longest = longest; s.tiles = tiles; s.packed = packed;
+        return plan_segments(s, backward);
+    });
     m.def("selective_scan_update", &selective_scan_update);
     m.def("short_conv_update", &short_conv_update);
     m.def("add_rms_norm", &add_rms_norm);

@@ -3,6 +3,8 @@ the CPU an accepted call ends with the runtime's error (there is no device, so t
 import pytest
 import torch
 
+from oracle.naive_kda import err_ratio
+from oracle.ssm import selective_scan_ref
 from tests.block_c import GARBAGE, ConvStepArgs, NormArgs, ScanArgs, StepArgs, call
 
 EINVAL, EALIGN = -1, -2
@@ -104,3 +106,62 @@ def test_workspaces_that_a_scan_does_not_use_are_not_written():
     assert call("selective_scan_bwd", ScanArgs(**base, **at(own), part_skip=spare.data_ptr(), part_bias=spare.data_ptr()), stream) == 0
     torch.cuda.synchronize()
     assert (spare == 7.0).all() and own["dA"].isfinite().all()
+
+
+def scan_through_c(a, cu, dy, dhT, seg_chunks, cta_rows):
+    """Forward and backward of one scan with segments and CTA rows as asked for; everything that is written is NaN before."""
+    from cula_b200 import _native
+    from cula_b200.utils import VarlenTables
+    lib, d = _native.lib(), {k: v.cuda().contiguous() if torch.is_tensor(v) else v for k, v in a.items()}
+    (n, T, D), (G, S), dtype = a["x"].shape, a["B"].shape[2:], a["x"].dtype
+    SP = next(p for p in (8, 16, 32, 64) if p >= S)
+    tab = None if cu is None else VarlenTables(cu.cuda())
+    n_seqs, chunks = (n, n * -(-T // 64)) if cu is None else (tab.n_seqs, tab.num_chunks)
+    slots = 0 if not seg_chunks else n_seqs * -(-(-(-T // 64)) // seg_chunks) if cu is None else chunks // seg_chunks + n_seqs
+    tiles = lib.cula_kda_selective_scan_tiles(D, G, S)
+    nan = lambda *s, t=torch.float32: torch.full(s, float("nan"), device="cuda", dtype=t)  # noqa: E731
+    out = dict(y=nan(n, T, D, t=dtype), hT=nan(n_seqs, D, S), dx=nan(n, T, D, t=dtype), ddt=nan(n, T, D, t=dtype), dz=nan(n, T, D, t=dtype),
+               dBm=nan(n, T, G, S, t=dtype), dCm=nan(n, T, G, S, t=dtype), dA=nan(D, S), dskip=nan(D), dbias=nan(D), dh0=nan(n_seqs, D, S))
+    work = dict(states=nan(chunks * 8, lib.cula_kda_selective_scan_state_floats(D, G, S)), y_pre=nan(n, T, D), part_bc=nan(tiles, n * T, G, 2, SP),
+                part_A=nan(cta_rows, D, SP), part_skip=nan(cta_rows, D), part_bias=nan(cta_rows, D), seg_state=nan(max(1, slots), D, SP), seg_dt=nan(max(1, slots), D))
+    up = dict(dy=dy.cuda(), dhT=dhT.cuda())
+    ins = dict(x=d["x"], dt=d["dt"], z=d["z"], Bm=d["B"], Cm=d["C"], A=d["A"], skip=d["D"], dt_bias=d["dt_bias"], h0=d["initial_state"])
+    tables = {} if cu is None else {k: getattr(tab, k).contiguous() for k in ("cu_seqlens", "chunk_offsets", "seq_order")}
+    args = ScanArgs(**{k: t.data_ptr() for k, t in {**out, **work, **up, **ins, **tables}.items()}, x_row=D, dt_row=D, z_row=D, b_row=G * S, c_row=G * S,
+                    x_seq=T * D, dt_seq=T * D, z_seq=T * D, b_seq=T * G * S, c_seq=T * G * S, rows=n * T, T=T, D=D, S=S, G=G, n_seqs=n_seqs, num_chunks=chunks,
+                    total_tokens=0 if cu is None else tab.total_tokens, seg_chunks=seg_chunks, cta_rows=cta_rows, softplus=1, fp32=dtype == torch.float32,
+                    vec_bc=S % 4 == 0)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert call("selective_scan_fwd", args, stream) == 0 and call("selective_scan_bwd", args, stream) == 0
+    torch.cuda.synchronize()
+    return {k: t.cpu() for k, t in out.items()}, slots
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,D,S,dtype,seg_chunks,cta_rows", [
+    ([70, 0, 130, 5, 0, 200, 64], 272, 5, "bf16", 0, 1), ([70, 0, 130, 5, 0, 200, 64], 272, 5, "fp32", 1, 2),
+    ([70, 0, 130, 5, 0, 200, 64], 144, 16, "fp32", 0, 2), ([70, 0, 130, 5, 0, 200, 64], 144, 16, "bf16", 1, 1), (None, 144, 16, "bf16", 2, 3),
+    ([70, 0, 130, 5, 0, 200, 64], 80, 32, "bf16", 0, 1), ([70, 0, 130, 5, 0, 200, 64], 80, 32, "fp32", 2, 2), (None, 80, 32, "fp32", 0, 2),
+    ([70, 0, 130, 5, 0, 200, 64], 48, 64, "fp32", 0, 2), ([70, 0, 130, 5, 0, 200, 64], 48, 64, "bf16", 1, 2), (None, 48, 64, "fp32", 1, 1)])
+def test_ctas_that_walk_several_sequences_or_segments(lens, D, S, dtype, seg_chunks, cta_rows):
+    """Two groups of two channel tiles (the second not whole), every gradient: what a CTA hands on from one item to the next, sums over items,
+    empty sequences between, segments of every state width. Tolerances as for whole calls (test_selective_scan.py)."""
+    from tests.test_selective_scan import in64, make, tol
+    dtype = torch.bfloat16 if dtype == "bf16" else torch.float32
+    cu = None if lens is None else torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    n, T = (5, 150) if cu is None else (1, int(cu[-1]))
+    N = n if cu is None else len(lens)
+    a = make(n, T, D, S, 2, dtype, h0=N, seed=S + seg_chunks)
+    gen = torch.Generator().manual_seed(3)
+    dy, dh = torch.randn(n, T, D, generator=gen).to(dtype), 0.1 * torch.randn(N, D, S, generator=gen)
+    got, slots = scan_through_c(a, cu, dy, dh, seg_chunks, cta_rows)
+    items = slots if seg_chunks else N
+    assert items >= 5 and items > cta_rows                          # the loop over items is entered again
+    if seg_chunks:
+        assert max(-(-(-(-k // 64)) // seg_chunks) for k in ([T] if lens is None else lens)) >= 2
+    r = in64(a, True)
+    y, fin = selective_scan_ref(**r, cu_seqlens=cu)
+    leaves = dict(dx="x", ddt="dt", dz="z", dBm="B", dCm="C", dA="A", dskip="D", dbias="dt_bias", dh0="initial_state")
+    ref = dict(zip(leaves, torch.autograd.grad([y, fin], [r[k] for k in leaves.values()], [dy.double(), dh.double()])), y=y.detach(), hT=fin.detach())
+    errors = {k: err_ratio(ref[k], got[k]) / tol(got[k].dtype, T) for k in ref}
+    assert all(e < 1 for e in errors.values()), errors

@@ -276,7 +276,63 @@ def test_capture_beside_a_living_eager_graph_is_refused():
         assert torch.equal(static, eager)
 
 
+# More rows than the blocks hold at once (148 SMs): blocks of 512, 256 and 128 threads walk several rows, or several groups of narrow rows, the last
+# of them not whole. Every row is compared.
+LOOPS = [(1500, 4096, "bf16", "none"), (1501, 4096, "bf16", "fp32"), (1300, 8192, "bf16", "bf16"), (1201, 8192, "bf16", "fp32"), (700, 12288, "bf16", "fp32"),
+         (40003, 64, "bf16", "fp32"), (20009, 128, "bf16", "bf16"), (6001, 520, "fp32", "fp32"), (3001, 2560, "bf16", "none")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,D,dtype,res", LOOPS)
+def test_norm_of_more_rows_than_blocks(R, D, dtype, res):
+    test_norm_matches_oracle(R, D, dtype, res)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,D,dtype,res,group", [(*n, g) for n in LOOPS for g in (None, 64) if g is None or n[1] % g == 0])
+def test_norm_in_8_bits_of_more_rows_than_blocks(R, D, dtype, res, group):
+    test_norm_in_8_bits(R, D, dtype, res, group)
+
+
+@pytest.mark.gpu
+def test_norm_and_conv_step_with_parameters_in_16_bits():
+    """The same results as with the parameters' values in 32 bits, and gradients in 16."""
+    from cula_b200.kda import add_rms_norm, add_rms_norm_fp8, short_conv_update
+    gen = torch.Generator().manual_seed(12)
+    x, r = torch.randn(20, 264, generator=gen).bfloat16().cuda(), torch.randn(20, 264, generator=gen).cuda()
+    w16 = (1 + 0.1 * torch.randn(264, generator=gen)).bfloat16().cuda().requires_grad_(True)
+    w32 = w16.detach().float().requires_grad_(True)
+    (y, v), (y2, v2) = add_rms_norm(x, w16, r), add_rms_norm(x, w32, r)
+    g, g2 = torch.autograd.grad(y, w16, torch.ones_like(y))[0], torch.autograd.grad(y2, w32, torch.ones_like(y))[0]
+    assert torch.equal(y, y2) and torch.equal(v, v2) and g.dtype == torch.bfloat16 and torch.equal(g, g2.bfloat16())
+    for a, b in zip(add_rms_norm_fp8(x, w16, r), add_rms_norm_fp8(x, w32, r)):
+        assert torch.equal(a.float(), b.float())
+    cw, b = torch.randn(264, 4, generator=gen).bfloat16().cuda(), torch.randn(264, generator=gen).bfloat16().cuda()
+    pools = [torch.randn(20, 264, 4, generator=gen).cuda()] * 2
+    pools = [p.clone() for p in pools]
+    assert torch.equal(short_conv_update(x, cw, pools[0], bias=b), short_conv_update(x, cw.float(), pools[1], bias=b.float())) and torch.equal(*pools)
+
+
 # ------------------------------------------------ short convolution, single tokens ------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,D,W", [(256, 12288, 4), (255, 12288, 3), (131, 8200, 2)])
+def test_conv_step_of_more_rows_than_blocks(N, D, W):
+    """Blocks walk five rows or more each; skipped sequences among the first, middle and last of them."""
+    from cula_b200.kda import check_status, short_conv_update
+    gen = torch.Generator().manual_seed(N)
+    rn = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, w, b, pool = rn(N, D).bfloat16(), 0.5 * rn(D, W), 0.1 * rn(D), rn(N + 2, D, W)
+    idx = torch.randperm(N + 2, generator=gen)[:N].to(torch.int32)
+    idx[[0, 7, N // 2, N // 2 + 1, N - 1]] = -1
+    y_ref, pool_ref = short_conv_update_ref(x.double(), w.double(), pool.double(), idx, b.double())
+    cache = pool.cuda()
+    y = short_conv_update(x.cuda(), w.cuda(), cache, idx.cuda(), b.cuda())
+    torch.cuda.synchronize()
+    check_status(torch.device("cuda", 0))
+    assert torch.equal(cache.cpu().double(), pool_ref) and (y.cpu()[idx < 0] == 0).all()
+    assert err_ratio(y_ref, y.double().cpu()) < BF16
+
+
 @pytest.mark.gpu
 def test_conv_step_in_a_pool_past_32_bits():
     from cula_b200.kda import short_conv_update

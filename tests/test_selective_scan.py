@@ -137,6 +137,24 @@ def test_c_entries_refuse_what_they_cannot_do():
     assert lib.cula_kda_add_rms_norm_shares(128, 0) == 0
 
 
+def chunks_of(T, lens):
+    return [-(-n // 64) for n in ([T] if lens is None else lens)]
+
+
+CUT = [(None, 1500, 40, 16), ([700, 0, 1000, 30, 129], 1900, 24, 12)]
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_few_channels_and_long_sequences_are_cut(backward):
+    """What the GPU test of cut sequences stands on; and many short sequences of many channels are not."""
+    from cula_b200 import _native
+    plan, tiles = _native.host().selective_scan_segments, _native.lib().cula_kda_selective_scan_tiles
+    for lens, T, D, S in CUT:
+        chunks = chunks_of(T, lens)
+        assert 0 < plan(len(chunks), sum(chunks), max(chunks), tiles(D, 1, S), lens is not None, backward) < max(chunks)
+    assert plan(64, 64 * 4, 4, tiles(4096, 1, 16), False, backward) == 0 and plan(1, 1, 1, 1, False, backward) == 0
+
+
 # ------------------------------------------------------------------ GPU ------------------------------------------------------------------
 def check_all(a, cu=None, want_final=True, seed=9, names=None):
     """Outputs and every gradient of a call against the oracle's."""
@@ -242,6 +260,22 @@ def test_errors_do_not_add_up_over_a_memory():
     g_got = torch.autograd.grad(got, [d[k] for k in leaves], [dy.cuda(), df.cuda()])
     errors = {k: err_ratio(u.detach(), v.detach().double().cpu()) for k, u, v in zip(["y", "fin"] + leaves, [*ref, *g_ref], [*got, *g_got])}
     assert all(e < 1.25e-6 for e in errors.values()), errors
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_a_bad_value_stays_in_its_channel(value):
+    """NaN or infinity in one live token of x: its channel from that token on, and no other channel, sequence or earlier token."""
+    from cula_b200.kda import selective_scan
+    a = on_gpu(make(2, 40, 72, 16, 1, torch.float32, h0=2, seed=31))
+    clean = selective_scan(**a, output_final_state=True)
+    a["x"][1, 21, 5] = value
+    y, fin = selective_scan(**a, output_final_state=True)
+    hit = torch.zeros(2, 40, 72, dtype=torch.bool, device="cuda")
+    hit[1, 21:, 5] = True
+    assert torch.equal(y[~hit], clean[0][~hit]) and not y[hit].isfinite().any()
+    assert torch.equal(fin[0], clean[1][0]) and torch.equal(fin[1, torch.arange(72) != 5], clean[1][1, torch.arange(72) != 5])
+    assert not fin[1, 5].isfinite().any()
 
 
 @pytest.mark.gpu
@@ -536,6 +570,21 @@ def test_step_matches_oracle(N, D, S, G, dtype, gate, indexed):
     touched = torch.zeros(N + 3, dtype=torch.bool)
     touched[(torch.arange(N) if idx is None else idx[idx >= 0]).long()] = True
     assert torch.equal(state.cpu()[~touched], pool[~touched])
+
+
+@pytest.mark.gpu
+def test_step_without_softplus_and_with_parameters_in_16_bits():
+    from cula_b200.kda import selective_scan_update
+    a = {k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in make(5, 1, 72, 16, 1, torch.float32, seed=6).items()}
+    del a["initial_state"]
+    a.update(dt_softplus=False, dt=0.05 * a["dt"].abs(), dt_bias=0.01 * torch.rand(72, generator=torch.Generator().manual_seed(1)))
+    for k in ("A", "D", "dt_bias"):
+        a[k] = a[k].bfloat16()
+    pool = torch.randn(5, 72, 16, generator=torch.Generator().manual_seed(2))
+    y_ref, pool_ref = selective_scan_update_ref(**in64(a), state=pool.double())
+    state = pool.cuda()
+    y = selective_scan_update(**on_gpu(a), state=state)
+    assert err_ratio(y_ref, y.double().cpu()) < tol(torch.float32, 1) and err_ratio(pool_ref, state.double().cpu()) < tol(torch.float32, 1)
 
 
 @pytest.mark.gpu
