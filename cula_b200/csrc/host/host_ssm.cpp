@@ -17,7 +17,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 constexpr int64_t KEEP = 8;                    // tokens per kept state
-constexpr int64_t SMS = 148;
+constexpr int64_t SMS = 148;                   // of a B200: the models below were fitted there
 
 bool grad_wanted(std::initializer_list<OptTensor> ts) {
     for (const OptTensor& t : ts)

@@ -4,7 +4,7 @@
 //     dv = rstd (dn - n mean(dn n)) + dr_out with dn = dy w;  dx, dr = dv;  dw = sum over rows of dy n
 // Everything is read and written once: TPR threads hold a row in registers, VPT pieces of 8 columns each, and ask for their next row before
 // they sum, scale and store this one. Bound by memory: 8192 x 4096 in bf16 forward 40 us (268 MB: 6.6 TB/s), backward 44 (268 MB), 8-bit output
-// beside an fp32 stream at 16384 x 4096 112 us (738 MB: 6.6 TB/s), 114 with a scale per 128 columns.
+// beside an fp32 stream at 16384 x 4096 112 to 117 us (738 MB: 6.3 to 6.6 TB/s), the same with a scale per 128 columns.
 #include <cuda_fp8.h>
 
 #include "kda_common.cuh"
@@ -74,7 +74,9 @@ __device__ __forceinline__ int row_max(int v, int* slot) {
 }
 
 // v / scale, as exact as a division: a product with the reciprocal alone is off by a rounding more, and puts twice as many values on the
-// other side of a boundary between two 8-bit values. The reciprocal has a second part, its own rounding.
+// other side of a boundary between two 8-bit values. The reciprocal has a second part, its own rounding. Of 2^26 values 35 to 48 are then not
+// the nearest to 64 bits' quotient, and 46 to 64 of plain fp32; with products and factor in two parts none would be, for twice the time of a
+// norm without a stream (46 -> 88 us at 16384 x 4096), or 63 us where only quotients beside a boundary are done so.
 struct Quotient {
     float inv, rest;
     __device__ Quotient(float scale) : inv(1.f / scale), rest(scale < INFINITY ? fmaf(-scale, inv, 1.f) * inv : 0.f) {}

@@ -120,7 +120,7 @@ __device__ __forceinline__ float2 sub2(float2 a, float2 b) { return make_float2(
 __device__ __forceinline__ float2 ex2_2(float2 a) { return make_float2(fast_exp2(a.x), fast_exp2(a.y)); }
 // What a recurrence over tokens decays by, 2^(d a). The unit's exponential is low by 2e-8 on average for exponents in (-1, -0.005), 5e-8 below
 // them and 5e-9 above, and a state takes in as many of these errors as it remembers tokens. The exponent's rounding is where they are
-// made up for, at no instruction more: the mean error is then within 1.5e-8 down to -1 (gradient of the rates at 4 x 2048 tokens: 2.0e-6
+// made up for, at no instruction more: the mean error is then within 1.6e-8 down to -1 (gradient of the rates at 4 x 2048 tokens: 2.0e-6
 // -> 1.1e-6). 2^0 stays 1.
 constexpr float DECAY_CENTRE = 2.2e-8f;
 __device__ __forceinline__ float decay(float d, float a) { return fast_exp2(fmaf(d, a, DECAY_CENTRE)); }

@@ -10,9 +10,10 @@
 //
 // Four warps scan, with the 136 registers that eight tokens' states and factors take, and four serve them as in the forward pass: rows two
 // tiles ahead, operands of the next tile, gradients of the tile before. Per element one exponential, eleven multiply-adds (packed in
-// pairs) and two sums over lanes, which go as half of the values per step. At 4 x 2048 x 4096 x 16 in bf16 with a gate (473 MB): 73 us of
-// traffic, 115 (145) us of exponentials, 184 us of multiply-adds at their rate. Measured: 1040 us with every thread doing everything, 566
-// so (lone CTAs 345). Nothing is saturated: issue slots 58 %, of which packed multiply-adds take two each, shared memory's data path 53 %
+// pairs) and two sums over lanes, which go as half of the values per step. At 4 x 2048 x 4096 x 16 in bf16 with a gate: 473 MB of inputs and
+// gradients (73 us) and 536 of kept states, y before the gate and shares of dB and dC there and back (83 us more), 115 us of the recurrence's
+// exponentials (165 with softplus and three sigmoids per token and channel), 184 us of multiply-adds at their rate. Measured: 1040 us with
+// every thread doing everything, 567 so (lone CTAs 345). Nothing is saturated: issue slots 58 %, of which packed multiply-adds take two each, shared memory's data path 53 %
 // of the launch; 22 % of the warps that would fit are resident, since registers and shared memory hold two CTAs per SM. Tried: sums over
 // channels by tensor-core products with ones (590: fewer exchanges, no less time), packed pairs over channels in place of states (689: B
 // and C twice in shared memory), eight scanning warps and four serving ones in one CTA per SM (617), other register splits (176 + 80: 592).
@@ -28,8 +29,8 @@ __device__ __forceinline__ void sel_bwd_barrier() { asm volatile("bar.sync 1, %0
 template <int SL, typename T>
 struct SelBwdSmem {
     using G = SelShape<SL>;
-    // tiles of rows: of the gradients that are made, of the next tile, one more of 16 bits where two CTAs still share an SM
-    // (64 states, 4 x 2048 x 4096: 2.88 ms with three, 2.13 with two)
+    // tiles of rows: of the gradients that are made, of the next tile, and one more where the rows are of 16 bits and two CTAs share an SM all
+    // the same (64 states, 4 x 2048 x 4096: 2.88 ms with three, 2.13 with two). With 64 states in fp32 one CTA has the SM either way.
     static constexpr int Q = SelVec<T>::Q, RING = Q == 1 && SL < 16 ? 3 : 2;
     float4 dx[2][G::LC][G::CH / 2];                                  // two channels' steps, and their products with x
     float2 dy[2][G::LC][G::CH / 2];

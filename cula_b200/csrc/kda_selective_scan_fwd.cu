@@ -4,8 +4,8 @@
 // once per token and channel, for the next tile, and turn the sums of the tile before into outputs. One barrier per tile.
 //
 // What it cannot do without at 4 x 2048 tokens x 4096 channels x 16 states in bf16 with a gate (268 MB): 42 us of HBM traffic, 115 us of
-// exponentials (16 per clock and SM), 145 with those of softplus and silu. Measured: 524 us with every thread staging, scanning and writing
-// in turn (B and C rows waited for in registers, 16-byte loads of 32 lanes to 32 lines for the kept states), 219 us so; 234 with the
+// exponentials (16 per clock and SM), 137 with the three of softplus and silu per token and channel. Measured: 524 us with every thread staging, scanning and writing
+// in turn (B and C rows waited for in registers, 16-byte loads of 32 lanes to 32 lines for the kept states), 219 us so; 235 with the
 // states kept for a backward pass. The unit of the exponentials is 66 % busy: 256 CTAs leave 40 of 148 SMs with one CTA in place of two
 // (86 %), and of a pair's time it is busy for three quarters; the data path of shared memory is half busy beside it. An eighth or a quarter
 // of the exponentials as polynomials on the multiply-add units made it 6 and 9 us slower.

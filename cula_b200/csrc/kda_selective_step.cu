@@ -79,7 +79,7 @@ __device__ __forceinline__ int step_slot(const int* indices, int row, int pool, 
 // channel as a whole (step, gate, output) is done by one lane, its owner, and handed to the others. The next row's states are on their way to
 // shared memory, each thread's to a place of its own, while a row is worked on; everything else is asked for one row ahead too.
 // Bound by memory: 256 rows x 4096 channels x 16 states in bf16 (143 MB, 22 us at the copy rate) take 65 us with a block per row and tile
-// and 27.8 so (5.1 TB/s, launch and ramp included; 512 rows 5.6). The next row in registers: 29.3, and 46 in the place of 28 where 64 states
+// and 28 to 29 so (5.0 TB/s, launch and ramp included; 512 rows 5.6). The next row in registers: 29.3, and 46 in the place of 28 where 64 states
 // leave none. Two rows ahead: 28.6; other numbers of blocks per SM: 30 to 35.
 constexpr int STEP_RING = 2;
 // Blocks that an SM holds: those of few states per channel need more of them for as many bytes on their way (8 states: 23 -> 19 us)
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(STEP_THREADS, step_resident(SL)) kda_selective
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// two neighbouring channels per thread; 256 rows x 12288 channels x 4 (113 MB, 17.6 us at the copy rate): 20.1 us
+// two neighbouring channels per thread; 256 rows x 12288 channels x 4 (113 MB, 17.6 us at the copy rate): 20.5 us
 template <int W>
 __global__ void __launch_bounds__(STEP_THREADS) kda_conv_step_kernel(const ConvStepArgs a, const int tiles, const int row_step) {
     const int d0 = 2 * ((blockIdx.x % tiles) * blockDim.x + threadIdx.x);

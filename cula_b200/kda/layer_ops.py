@@ -49,7 +49,8 @@ def short_conv_update(x, weight, cache, cache_indices=None, bias=None, activatio
     ``[pool, D, W]`` fp32, contiguous: the last ``W`` inputs of each slot, newest last (what ``short_conv`` returns as its final
     state); each used window takes in its token, in place. cache_indices: ``[N]`` int32 slots, negative = skip the sequence (zero
     output, no access to the pool), or None for slot = sequence; a slot may be named once in a call. A slot past the pool is skipped
-    too and reported by ``check_status``. Returns ``y`` shaped like x (``out`` if given). No gradients."""
+    too and reported by ``check_status``. Returns ``y`` shaped like x (``out`` if given). No gradients, and tangents are refused;
+    autograd knows that cache and out were written to."""
     assert activation in (None, "silu", "swish"), "activation must be None, 'silu' or 'swish'."
     return _native.host().short_conv_update(x, weight, cache, cache_indices, bias, activation is not None, out)
 
@@ -71,7 +72,8 @@ def add_rms_norm_fp8(x, weight, residual=None, eps=1e-6, group_size=None):
     rounding of q.
 
     ``scale`` is fp32, ``max(amax / 448, 2^-126)`` over each row (``group_size`` None: ``[...]``) or over each ``group_size``
-    (32, 64, 128 or 256) neighbouring columns (``[..., D / group_size]``); ``q`` is ``torch.float8_e4m3fn``. A row that holds a NaN or
-    an infinity has NaN there. Other arguments as for ``add_rms_norm``. No gradients."""
+    (32, 64, 128 or 256) neighbouring columns (``[..., D / group_size]``); ``q`` is ``torch.float8_e4m3fn``. A row that holds a
+    NaN is NaN in all of q and scale; one that holds an infinity is NaN where its scale covers the infinity, and zero in other groups (all else
+    is divided by an infinite norm). Other arguments as for ``add_rms_norm``. No gradients, and tangents are refused."""
     q, scale, v = _native.host().add_rms_norm_fp8(x, weight, residual, eps, 0 if group_size is None else group_size)
     return q, scale, x if v is None else v
